@@ -201,4 +201,84 @@ constexpr size_t kAmaxCounterBytes = (kSchedQueueStride + 1) * sizeof(uint32_t);
 hipError_t launch_tensor_scales(const WriteLaunch& l, bool bf16, float* k_scale, float* v_scale,
                                 uint32_t* counter, uint32_t* partials);
 
+// Rows into (write) or out of (gather) the 4-bit paged cache (pa_int4_rows.hip).
+struct Int4Rows {
+  void* key;      // read by the write, written by the gather; 16-bit elements
+  void* value;
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  const int64_t* slot_mapping;
+  int num_tokens;
+  int num_kv_heads;
+  int head_dim;
+  void* k_cache;
+  void* v_cache;
+  void* k_scales;   // fp16 (scale, minimum) pairs
+  void* v_scales;
+  int num_blocks;
+  int block_size;
+  bool bf16;
+  hipStream_t stream;
+};
+hipError_t launch_int4_write(const Int4Rows& l);
+hipError_t launch_int4_gather(const Int4Rows& l);
+
+// Decode over the 4-bit paged cache (pa_decode_int4.hip).
+struct Int4DecodeShape {
+  int num_seqs;
+  int num_heads;
+  int num_kv_heads;
+  int group;        // num_heads / num_kv_heads
+  int head_dim;
+  int num_blocks;
+  int max_blocks;   // block_table row stride
+  int bs_log2;
+  float scale_log2; // softmax scale * log2(e)
+};
+struct Int4Decode {
+  void* out;
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const void* k_scales;
+  const void* v_scales;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  bool bf16;           // q and out
+  uint32_t* counters;  // int4_decode_counter_bytes(), zero between launches
+  float* workspace;    // int4_decode_workspace_bytes(shape)
+  Int4DecodeShape shape;
+  hipStream_t stream;
+};
+hipError_t launch_int4_decode(const Int4Decode& l);
+size_t int4_decode_workspace_bytes(const Int4DecodeShape& s);
+size_t int4_decode_counter_bytes();
+
+// Block tables, slots and positions of new tokens (pa_block_tables.hip).
+constexpr int kExtendMaxSeqs = 4096;
+constexpr int kExtendNoBlocks = 1, kExtendRowFull = 2, kExtendNoRows = 4, kExtendBadLength = 8;
+struct ExtendLaunch {
+  int32_t* block_table;
+  const int32_t* context_lens;
+  const int32_t* new_lens;
+  const int32_t* free_blocks;
+  const int32_t* num_free;
+  int32_t* context_lens_out;
+  int32_t* num_free_out;
+  int64_t* slot_mapping;
+  int64_t* positions;     // may be NULL
+  int32_t* cu_seqlens;    // may be NULL
+  int32_t* status;
+  uint32_t* counter;      // one word, zero between launches
+  int num_seqs;
+  int max_blocks;
+  int block_size;
+  int num_rows;
+  int free_capacity;
+  hipStream_t stream;
+};
+hipError_t launch_extend(const ExtendLaunch& l);
+
 }  // namespace pa

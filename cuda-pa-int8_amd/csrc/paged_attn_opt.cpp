@@ -375,6 +375,197 @@ std::pair<int64_t, int64_t> decode_plan(int64_t kind, int64_t num_seqs, int64_t 
   return {part, ns};
 }
 
+// ---- the 4-bit paged cache (layout: include/pa_mi355x.h)
+
+// Shapes, dtypes and devices of a 4-bit cache's four tensors, against rows or queries `like`
+// of `kv_heads` (0: any) heads of head_dim `d`.
+void check_int4_cache(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                      const at::Tensor& k_scales, const at::Tensor& v_scales,
+                      const at::Tensor& like, int64_t kv_heads, int64_t d) {
+  TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
+              "k_cache and v_cache must be uint8");
+  TORCH_CHECK(k_scales.scalar_type() == at::kHalf && v_scales.scalar_type() == at::kHalf,
+              "scales must be fp16");
+  TORCH_CHECK(k_cache.dim() == 6 && k_cache.size(4) == 4 && k_cache.size(5) == 4 &&
+                  v_cache.sizes() == k_cache.sizes(),
+              "4-bit caches must be [blocks, kv_heads, block_size / 4, head_dim / 8, 4, 4]");
+  TORCH_CHECK(k_cache.size(3) * 8 == d && (kv_heads == 0 || k_cache.size(1) == kv_heads),
+              "cache shapes do not match kv_heads / head_dim");
+  TORCH_CHECK(k_scales.dim() == 4 && k_scales.size(0) == k_cache.size(0) &&
+                  k_scales.size(1) == k_cache.size(1) && k_scales.size(2) == 4 * k_cache.size(2) &&
+                  k_scales.size(3) == 2 && v_scales.sizes() == k_scales.sizes(),
+              "scales must be [blocks, kv_heads, block_size, 2]");
+  for (const at::Tensor* t : {&k_cache, &v_cache, &k_scales, &v_scales})
+    TORCH_CHECK(t->is_contiguous() && t->is_cuda() && t->get_device() == like.get_device(),
+                "cache tensors must be contiguous and on the rows' device");
+  TORCH_CHECK(k_cache.size(0) <= INT32_MAX, "too many blocks");
+}
+
+// Decode over the 4-bit cache; q and out fp16 or bf16.
+void paged_decode_attn_int4(at::Tensor out, at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
+                            at::Tensor k_scales, at::Tensor v_scales, at::Tensor block_table,
+                            at::Tensor context_lens, double scale, int64_t block_size,
+                            bool check_context) {
+  TORCH_CHECK(q.is_cuda() && out.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+              "q must be fp16 or bf16");
+  TORCH_CHECK(q.dim() == 3 && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(),
+              "q and out must be [num_seqs, num_heads, head_dim] of one dtype");
+  check_int4_cache(k_cache, v_cache, k_scales, v_scales, q, 0, q.size(2));
+  TORCH_CHECK(k_scales.size(2) == block_size, "cache block dimension must equal block_size");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt, "block_table must be int32");
+  TORCH_CHECK(context_lens.scalar_type() == at::kInt, "context_lens must be int32");
+  TORCH_CHECK(block_table.dim() == 2 && context_lens.dim() == 1 &&
+                  block_table.size(0) == q.size(0) && context_lens.size(0) == q.size(0),
+              "block_table must be [num_seqs, max_blocks] and context_lens [num_seqs]");
+  for (const at::Tensor* t : {&out, &q, &block_table, &context_lens}) {
+    TORCH_CHECK(t->is_cuda() && t->get_device() == q.get_device(), "all tensors must be on q's device");
+    TORCH_CHECK(t->is_contiguous(), "all tensors must be contiguous");
+  }
+  TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && block_table.size(1) <= INT32_MAX,
+              "q or block_table too large");
+  if (check_context && context_lens.numel() > 0) {
+    int32_t mn = 0, mx = 0, mean = 0;
+    if (!polled_range(context_lens, q, &mn, &mx, &mean)) mn = context_lens.min().item<int32_t>();
+    TORCH_CHECK(mn >= 1, "context_lens must be >= 1 (empty sequences unsupported)");
+  }
+  const int32_t S = (int32_t)q.size(0), H = (int32_t)q.size(1), D = (int32_t)q.size(2);
+  const int32_t Hkv = (int32_t)k_cache.size(1), MB = (int32_t)block_table.size(1);
+  const at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  hipStream_t stream = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.get_device()).stream();
+  const size_t need = pa_decode_int4_workspace_bytes(S, H, D, Hkv, (int32_t)block_size, MB);
+  at::Tensor cnt = counters_for(q, stream, pa_decode_int4_counter_bytes());
+  at::Tensor ws = at::empty({(int64_t)std::max<size_t>(need, 256)}, q.options().dtype(at::kByte));
+  check_status(pa_paged_decode_attn_int4(
+      out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
+      v_scales.data_ptr(), block_table.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
+      (float)scale, (int32_t)block_size, S, H, D, Hkv, (int32_t)k_cache.size(0), MB,
+      q.scalar_type() == at::kBFloat16, cnt.data_ptr(), cnt.numel(), ws.data_ptr(), ws.numel(),
+      reinterpret_cast<pa_stream_t>(stream)));
+}
+
+void check_int4_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_cache,
+                     const at::Tensor& v_cache, const at::Tensor& k_scales,
+                     const at::Tensor& v_scales, const at::Tensor& slot_mapping) {
+  TORCH_CHECK(key.is_cuda() && value.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK((key.scalar_type() == at::kHalf || key.scalar_type() == at::kBFloat16) &&
+                  value.scalar_type() == key.scalar_type(),
+              "key and value must be fp16 or bf16 (the same)");
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kLong, "slot_mapping must be int64");
+  TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes(),
+              "key and value must be [num_tokens, num_kv_heads, head_dim]");
+  TORCH_CHECK(key.stride(2) == 1 && value.stride(2) == 1, "head_dim must be the innermost dim");
+  TORCH_CHECK(value.get_device() == key.get_device(), "key and value must be on one device");
+  check_int4_cache(k_cache, v_cache, k_scales, v_scales, key, key.size(1), key.size(2));
+  TORCH_CHECK(slot_mapping.dim() == 1 && slot_mapping.size(0) == key.size(0),
+              "slot_mapping must be [num_tokens]");
+  TORCH_CHECK(slot_mapping.is_contiguous() && slot_mapping.is_cuda() &&
+                  slot_mapping.get_device() == key.get_device(),
+              "slot_mapping must be contiguous and on the rows' device");
+  TORCH_CHECK(key.size(0) <= INT32_MAX, "too many tokens");
+}
+
+// Quantize + paged write of fp16 or bf16 key / value into the 4-bit cache.
+void reshape_and_cache_int4(at::Tensor key, at::Tensor value, at::Tensor k_cache,
+                            at::Tensor v_cache, at::Tensor k_scales, at::Tensor v_scales,
+                            at::Tensor slot_mapping) {
+  check_int4_rows(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping);
+  const at::hip::HIPGuardMasqueradingAsCUDA guard(key.device());
+  hipStream_t stream = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(key.get_device()).stream();
+  check_status(pa_reshape_and_cache_int4(
+      key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0),
+      value.stride(1), slot_mapping.data_ptr<int64_t>(), (int32_t)key.size(0),
+      (int32_t)key.size(1), (int32_t)key.size(2), k_cache.data_ptr(), v_cache.data_ptr(),
+      k_scales.data_ptr(), v_scales.data_ptr(), (int32_t)k_cache.size(0),
+      (int32_t)k_scales.size(2), key.scalar_type() == at::kBFloat16,
+      reinterpret_cast<pa_stream_t>(stream)));
+}
+
+// Whether no two rows of [tokens, heads, head_dim] share memory, in either order of the outer
+// dims (rows written at once must not).
+bool rows_disjoint(const at::Tensor& t) {
+  const bool heads_inner = t.size(0) < 2 || (t.size(1) > 1 && t.stride(1) <= t.stride(0));
+  const int in = heads_inner ? 1 : 0, out = 1 - in;
+  const int64_t d = t.size(2);
+  return t.numel() == 0 || ((t.size(in) == 1 || t.stride(in) >= d) &&
+                            (t.size(out) == 1 ||
+                             t.stride(out) >= (t.size(in) - 1) * t.stride(in) + d));
+}
+
+// The values of cached 4-bit rows into key / value (fp16 or bf16).
+void gather_cache_int4(at::Tensor key, at::Tensor value, at::Tensor k_cache, at::Tensor v_cache,
+                       at::Tensor k_scales, at::Tensor v_scales, at::Tensor slot_mapping) {
+  check_int4_rows(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping);
+  for (const at::Tensor* t : {&key, &value})
+    TORCH_CHECK(rows_disjoint(*t), "the rows of key and value must not overlap");
+  const at::hip::HIPGuardMasqueradingAsCUDA guard(key.device());
+  hipStream_t stream = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(key.get_device()).stream();
+  check_status(pa_gather_cache_int4(
+      key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0),
+      value.stride(1), slot_mapping.data_ptr<int64_t>(), (int32_t)key.size(0),
+      (int32_t)key.size(1), (int32_t)key.size(2), k_cache.data_ptr(), v_cache.data_ptr(),
+      k_scales.data_ptr(), v_scales.data_ptr(), (int32_t)k_cache.size(0),
+      (int32_t)k_scales.size(2), key.scalar_type() == at::kBFloat16,
+      reinterpret_cast<pa_stream_t>(stream)));
+}
+
+// Blocks, slots and positions for a batch's new tokens (pa_extend_block_tables).
+void extend_block_tables(at::Tensor block_table, at::Tensor context_lens, at::Tensor new_lens,
+                         at::Tensor free_blocks, at::Tensor num_free, at::Tensor slot_mapping,
+                         c10::optional<at::Tensor> positions, c10::optional<at::Tensor> cu_seqlens,
+                         at::Tensor status, int64_t block_size,
+                         c10::optional<at::Tensor> context_lens_out,
+                         c10::optional<at::Tensor> num_free_out) {
+  const at::Tensor& ctx_out = context_lens_out.has_value() ? *context_lens_out : context_lens;
+  const at::Tensor& free_out = num_free_out.has_value() ? *num_free_out : num_free;
+  TORCH_CHECK(block_table.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK(block_table.dim() == 2, "block_table must be [num_seqs, max_blocks]");
+  const int64_t S = block_table.size(0);
+  using Tensors = std::vector<const at::Tensor*>;
+  for (const at::Tensor* t : Tensors{&block_table, &context_lens, &new_lens, &free_blocks,
+                                     &num_free, &ctx_out, &free_out, &status})
+    TORCH_CHECK(t->scalar_type() == at::kInt, "block tables, lengths, free list and status must be int32");
+  for (const at::Tensor* t : Tensors{&context_lens, &new_lens, &ctx_out})
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == S, "lengths must be [num_seqs]");
+  for (const at::Tensor* t : Tensors{&num_free, &free_out, &status})
+    TORCH_CHECK(t->numel() == 1, "num_free and status must hold one value");
+  TORCH_CHECK(free_blocks.dim() == 1, "free_blocks must be one-dimensional");
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 1,
+              "slot_mapping must be int64 [rows]");
+  Tensors all = {&block_table, &context_lens, &new_lens, &free_blocks, &num_free,
+                 &slot_mapping, &status, &ctx_out, &free_out};
+  if (positions.has_value()) {
+    TORCH_CHECK(positions->scalar_type() == at::kLong && positions->sizes() == slot_mapping.sizes(),
+                "positions must be int64 [rows]");
+    all.push_back(&*positions);
+  }
+  if (cu_seqlens.has_value()) {
+    TORCH_CHECK(cu_seqlens->scalar_type() == at::kInt && cu_seqlens->dim() == 1 &&
+                    cu_seqlens->size(0) == S + 1,
+                "cu_seqlens must be int32 [num_seqs + 1]");
+    all.push_back(&*cu_seqlens);
+  }
+  for (const at::Tensor* t : all)
+    TORCH_CHECK(t->is_contiguous() && t->is_cuda() && t->get_device() == block_table.get_device(),
+                "all tensors must be contiguous and on block_table's device");
+  TORCH_CHECK(S <= PA_EXTEND_MAX_SEQS, "at most ", PA_EXTEND_MAX_SEQS, " sequences");
+  TORCH_CHECK(block_table.size(1) <= INT32_MAX && free_blocks.size(0) <= INT32_MAX &&
+                  slot_mapping.size(0) <= INT32_MAX, "too large");
+  const at::hip::HIPGuardMasqueradingAsCUDA guard(block_table.device());
+  hipStream_t stream =
+      at::hip::getCurrentHIPStreamMasqueradingAsCUDA(block_table.get_device()).stream();
+  at::Tensor cnt = counters_for(block_table, stream, kMinCounterBytes);
+  check_status(pa_extend_block_tables(
+      block_table.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
+      new_lens.data_ptr<int32_t>(), free_blocks.data_ptr<int32_t>(), num_free.data_ptr<int32_t>(),
+      ctx_out.data_ptr<int32_t>(), free_out.data_ptr<int32_t>(), slot_mapping.data_ptr<int64_t>(),
+      positions.has_value() ? positions->data_ptr<int64_t>() : nullptr,
+      cu_seqlens.has_value() ? cu_seqlens->data_ptr<int32_t>() : nullptr,
+      status.data_ptr<int32_t>(), (int32_t)S, (int32_t)block_table.size(1), (int32_t)block_size,
+      (int32_t)slot_mapping.size(0), (int32_t)free_blocks.size(0), cnt.data_ptr(), cnt.numel(),
+      reinterpret_cast<pa_stream_t>(stream)));
+}
+
 // Checks shared by the cache-write ops; `int8` selects the cache dtypes and
 // whether scale tensors are passed.
 void check_write(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_cache,
@@ -550,6 +741,14 @@ PYBIND11_MODULE(paged_attn_opt, m) {
   m.def("cache_prefill", &cache_prefill,
         "one prompt's cache write with the rest of its last block zeroed; per-tensor scales "
         "taken from the rows when asked for (new op)");
+  m.def("paged_decode_attn_int4", &paged_decode_attn_int4,
+        "paged decode over the 4-bit cache (fp16 or bf16 queries), optional host check (new op)");
+  m.def("reshape_and_cache_int4", &reshape_and_cache_int4,
+        "4-bit quantize + paged cache write (new op)");
+  m.def("gather_cache_int4", &gather_cache_int4,
+        "values of cached 4-bit rows, dequantized (new op)");
+  m.def("extend_block_tables", &extend_block_tables,
+        "blocks from the free list, slots and positions for a batch's new tokens (new op)");
   m.def("_length_slot", [](int refuse) {
     LengthSlot& s = length_slot();
     std::lock_guard<std::mutex> lk(s.mu);

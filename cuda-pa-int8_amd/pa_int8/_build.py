@@ -43,10 +43,13 @@ HIP_SOURCES = [
     "pa_ctx_range.hip",
     "pa_fill.hip",
     "pa_noalloc.hip",
+    "pa_int4_rows.hip",
+    "pa_decode_int4.hip",
+    "pa_block_tables.hip",
 ]
 # pa_quant.hip is compiled once per (scale mode, input type).
 QUANT_VARIANTS = tuple((given, bf16) for given in (0, 1) for bf16 in (0, 1))
-HOST_SOURCES = ["pa_capi.cpp"]
+HOST_SOURCES = ["pa_capi.cpp", "pa_capi_int4.cpp"]
 PROBE_SOURCES = ["bench/pa_probe.hip", "bench/pa_probe_decode.hip", "bench/pa_probe_write.hip"]
 
 HIPCC_FLAGS = [

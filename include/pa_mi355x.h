@@ -314,6 +314,84 @@ pa_status_t pa_cache_prefill(pa_cache_mode_t mode, int32_t bf16_input, const voi
                              size_t counter_bytes, void* workspace, size_t workspace_bytes,
                              pa_stream_t stream);
 
+/* ---- 4-bit paged cache.  NEW API (the reference has no 4-bit form).
+ *
+ * A row x of one (token, kv head), K and V alike, is held as head_dim codes c in 0..15 and
+ * an fp16 pair (scale s, minimum m) that stand for the values s * c + m:
+ *   m = fp16(min x), s = fp16((max x - min x) / 15), both saturated at fp16's largest;
+ *   c = clamp(rne((x - m) / s), 0, 15), 0 where s = 0.
+ * A row that holds an infinity or a NaN reads back as NaN.
+ *   k_cache, v_cache    uint8 [num_blocks, num_kv_heads, block_size / 4, head_dim / 8, 4, 4]:
+ *                       4 tokens of 8 dims in 16 bytes, dim e of a token in bits 4e .. 4e + 3
+ *   k_scales, v_scales  fp16 [num_blocks, num_kv_heads, block_size, 2]
+ * head_dim is a multiple of 8 in [8, 256], block_size 16, 32, 64 or 128.  Rows outside the
+ * cache are fp16, or bf16 where the call's bf16 flag is not 0, with strides and bases as
+ * pa_reshape_and_cache_int8 takes them; caches and scales are 16-byte aligned. */
+
+/* Quantizing write: the rows at slot_mapping (rules as pa_reshape_and_cache_int8; two tokens
+ * with the same slot leave that slot's contents unspecified). */
+pa_status_t pa_reshape_and_cache_int4(
+    const void* key, const void* value, int64_t key_token_stride, int64_t key_head_stride,
+    int64_t value_token_stride, int64_t value_head_stride, const int64_t* slot_mapping,
+    int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+    void* k_cache, void* v_cache, void* k_scales, void* v_scales,
+    int32_t num_blocks, int32_t block_size, int32_t bf16_input, pa_stream_t stream);
+
+/* The inverse: the values of the rows at slot_mapping into key and value, which a prompt
+ * chunk that continues a cached prefix attends over.  A slot outside the pool gives a row
+ * of zeros. */
+pa_status_t pa_gather_cache_int4(
+    void* key, void* value, int64_t key_token_stride, int64_t key_head_stride,
+    int64_t value_token_stride, int64_t value_head_stride, const int64_t* slot_mapping,
+    int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+    const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+    int32_t num_blocks, int32_t block_size, int32_t bf16_output, pa_stream_t stream);
+
+/* Decode over the 4-bit cache: q and out fp16, or bf16 where `bf16` is not 0; block table,
+ * lengths and behaviour on data the host cannot see as the other decode entry points.  The
+ * work is distributed on the device from context_lens.  `counters` as theirs (and may be
+ * shared with them); `workspace` is plain scratch. */
+size_t pa_decode_int4_counter_bytes(void);
+size_t pa_decode_int4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t head_dim,
+                                      int32_t num_kv_heads, int32_t block_size,
+                                      int32_t max_blocks_per_seq);
+pa_status_t pa_paged_decode_attn_int4(
+    void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+    const void* v_scales, const int32_t* block_table, const int32_t* context_lens, float scale,
+    int32_t block_size, int32_t num_seqs, int32_t num_heads, int32_t head_dim,
+    int32_t num_kv_heads, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t bf16,
+    void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
+    pa_stream_t stream);
+
+/* Room for a batch's new tokens.  NEW API: what a serving loop does on the host between
+ * steps, in one launch and without a read-back, for any cache type.  Sequence s holds
+ * context_lens[s] tokens and gets new_lens[s] more (both >= 0):
+ *   - each further block it needs is popped from the free list, the stack free_blocks[0 ..
+ *     *num_free), last entry first, sequence by sequence, and entered in its row of block_table;
+ *   - new token i of sequence s is token row cu_seqlens[s] + i: slot_mapping and positions
+ *     [num_rows] receive its slot and its position context_lens[s] + i.  Rows behind the last
+ *     token get slot -1, which the cache writes skip, and position 0;
+ *   - cu_seqlens [num_seqs + 1] receives the first row of each sequence and their number,
+ *     context_lens_out the new lengths, *num_free_out what is left (either may be the input:
+ *     updated in place).
+ * *status receives 0, or the sum of the reasons below; then nothing was placed: block_table,
+ * the lengths and the free count keep their values, and every row has slot -1.
+ * positions and cu_seqlens may be NULL.  block_size is a power of two up to 128,
+ * free_capacity the entries of free_blocks.  `counters`: 4 bytes or more under the rules of
+ * the decode counters, and shareable with them. */
+#define PA_EXTEND_MAX_SEQS 4096
+#define PA_EXTEND_NO_BLOCKS 1   /* fewer free blocks than needed */
+#define PA_EXTEND_ROW_FULL 2    /* a sequence longer than its row of the block table */
+#define PA_EXTEND_NO_ROWS 4     /* more new tokens than num_rows */
+#define PA_EXTEND_BAD_LENGTH 8  /* a negative length, or *num_free outside [0, free_capacity] */
+pa_status_t pa_extend_block_tables(
+    int32_t* block_table, const int32_t* context_lens, const int32_t* new_lens,
+    const int32_t* free_blocks, const int32_t* num_free, int32_t* context_lens_out,
+    int32_t* num_free_out, int64_t* slot_mapping, int64_t* positions, int32_t* cu_seqlens,
+    int32_t* status, int32_t num_seqs, int32_t max_blocks_per_seq, int32_t block_size,
+    int32_t num_rows, int32_t free_capacity, void* counters, size_t counter_bytes,
+    pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
