@@ -62,6 +62,26 @@ pa_status_t decode_shape(int32_t num_seqs, int32_t num_heads, int32_t head_dim,
   return PA_OK;
 }
 
+hipError_t launch_decode(const pa::Int4Decode& l) {
+  switch ((l.shape.head_dim + 31) / 32) {
+#define PA_CASE(N) \
+  case N: return pa::launch_int4_decode_steps<N>(l);
+    PA_FOR_EACH_INT4_STEPS(PA_CASE)
+#undef PA_CASE
+    default: return hipErrorInvalidValue;
+  }
+}
+
+size_t workspace_bytes_of(const pa::Int4DecodeShape& s) {
+  switch ((s.head_dim + 31) / 32) {
+#define PA_CASE(N) \
+  case N: return 2 * pa::kInt4Groups * pa::int4_decode_slot_bytes<N>(s.group);
+    PA_FOR_EACH_INT4_STEPS(PA_CASE)
+#undef PA_CASE
+    default: return 0;
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -94,7 +114,7 @@ pa_status_t pa_gather_cache_int4(void* key, void* value, int64_t key_token_strid
                    block_size, bf16_output, stream);
 }
 
-size_t pa_decode_int4_counter_bytes(void) { return pa::int4_decode_counter_bytes(); }
+size_t pa_decode_int4_counter_bytes(void) { return 3 * pa::kInt4Groups * sizeof(uint32_t); }
 
 size_t pa_decode_int4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t head_dim,
                                       int32_t num_kv_heads, int32_t block_size,
@@ -103,7 +123,7 @@ size_t pa_decode_int4_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32
   if (decode_shape(num_seqs, num_heads, head_dim, num_kv_heads, 1, block_size, max_blocks_per_seq,
                    1.f, &s) != PA_OK)
     return 0;
-  return pa::int4_decode_workspace_bytes(s);
+  return workspace_bytes_of(s);
 }
 
 pa_status_t pa_paged_decode_attn_int4(
@@ -122,14 +142,13 @@ pa_status_t pa_paged_decode_attn_int4(
     return PA_ERR_NULL_POINTER;
   for (const void* p : {static_cast<const void*>(out), q, k_cache, v_cache, k_scales, v_scales})
     if (!aligned(p, 16)) return PA_ERR_BAD_SHAPE;
-  if (!counters || counter_bytes < pa::int4_decode_counter_bytes() || !aligned(counters, 256) ||
-      workspace_bytes < pa::int4_decode_workspace_bytes(s) ||
-      (pa::int4_decode_workspace_bytes(s) > 0 && (!workspace || !aligned(workspace, 256))))
+  if (!counters || counter_bytes < pa_decode_int4_counter_bytes() || !aligned(counters, 256) ||
+      !workspace || workspace_bytes < workspace_bytes_of(s) || !aligned(workspace, 256))
     return PA_ERR_WORKSPACE;
   pa::Int4Decode l{out, q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens,
                    bf16 != 0, static_cast<uint32_t*>(counters), static_cast<float*>(workspace), s,
                    reinterpret_cast<hipStream_t>(stream)};
-  return pa::launch_int4_decode(l) == hipSuccess ? PA_OK : PA_ERR_LAUNCH;
+  return launch_decode(l) == hipSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
 pa_status_t pa_extend_block_tables(int32_t* block_table, const int32_t* context_lens,

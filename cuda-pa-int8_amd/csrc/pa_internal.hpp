@@ -247,14 +247,26 @@ struct Int4Decode {
   const int32_t* block_table;
   const int32_t* context_lens;
   bool bf16;           // q and out
-  uint32_t* counters;  // int4_decode_counter_bytes(), zero between launches
-  float* workspace;    // int4_decode_workspace_bytes(shape)
+  uint32_t* counters;  // 3 * kInt4Groups, zero between launches
+  float* workspace;    // 2 * kInt4Groups pieces
   Int4DecodeShape shape;
   hipStream_t stream;
 };
-hipError_t launch_int4_decode(const Int4Decode& l);
-size_t int4_decode_workspace_bytes(const Int4DecodeShape& s);
-size_t int4_decode_counter_bytes();
+constexpr int kInt4Groups = 256;   // work-groups of a launch, at most
+// Per number of 32-dim steps of a head (compiled with -DPA_INT4_STEPS): the launcher, and the
+// bytes of one piece in the workspace, which holds two for each work-group.
+template <int STEPS>
+hipError_t launch_int4_decode_steps(const Int4Decode& l);
+template <int STEPS>
+size_t int4_decode_slot_bytes(int group);
+#define PA_FOR_EACH_INT4_STEPS(X) X(1) X(2) X(3) X(4) X(5) X(6) X(7) X(8)
+#define PA_DECLARE_INT4_STEPS(N)                                  \
+  template <>                                                     \
+  hipError_t launch_int4_decode_steps<N>(const Int4Decode& l);    \
+  template <>                                                     \
+  size_t int4_decode_slot_bytes<N>(int group);
+PA_FOR_EACH_INT4_STEPS(PA_DECLARE_INT4_STEPS)
+#undef PA_DECLARE_INT4_STEPS
 
 // Block tables, slots and positions of new tokens (pa_block_tables.hip).
 constexpr int kExtendMaxSeqs = 4096;

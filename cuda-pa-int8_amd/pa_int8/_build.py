@@ -44,11 +44,13 @@ HIP_SOURCES = [
     "pa_fill.hip",
     "pa_noalloc.hip",
     "pa_int4_rows.hip",
-    "pa_decode_int4.hip",
     "pa_block_tables.hip",
 ]
 # pa_quant.hip is compiled once per (scale mode, input type).
 QUANT_VARIANTS = tuple((given, bf16) for given in (0, 1) for bf16 in (0, 1))
+# pa_decode_int4.hip is compiled once per number of 32-dim steps of a head (keep in step with
+# PA_FOR_EACH_INT4_STEPS in csrc/pa_internal.hpp).
+INT4_STEPS = tuple(range(1, 9))
 HOST_SOURCES = ["pa_capi.cpp", "pa_capi_int4.cpp"]
 PROBE_SOURCES = ["bench/pa_probe.hip", "bench/pa_probe_decode.hip", "bench/pa_probe_write.hip"]
 
@@ -115,6 +117,10 @@ def build_library(verbose=False, jobs=None):
         objs.append(obj)
         cmds.append(_compile_cmd("pa_quant.hip", obj,
                                  [f"-DPA_QUANT_GIVEN={given}", f"-DPA_QUANT_BF16={bf16}"]))
+    for n in INT4_STEPS:
+        obj = os.path.join(OBJ_DIR, f"pa_decode_int4_{n}.o")
+        objs.append(obj)
+        cmds.append(_compile_cmd("pa_decode_int4.hip", obj, [f"-DPA_INT4_STEPS={n}"]))
     for src in HIP_SOURCES + HOST_SOURCES:
         obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
         objs.append(obj)
