@@ -43,29 +43,21 @@ namespace pa {
 constexpr int kI4Waves = 8;          // waves of a work-group
 constexpr int kI4Groups = kInt4Groups;   // work-groups of a launch, at most: one a CU
 constexpr int kI4Tile = 64;          // tokens
-constexpr int kI4MinTiles = 2;       // tiles of a wave before another work-group is used
+constexpr int kI4MinTiles = 1;       // tiles of a wave before another work-group is used
 constexpr int kMergeMax = 16;        // pieces merged at once
 constexpr float kShift = 14.f;
+constexpr float kSlack = 1.5f;
 constexpr float kCode24 = 16777216.f;   // 2^24: a code's element times this is the code
 
+// What a launch knows beside its pointers.
 struct I4Args {
-  const uint16_t* q;
-  uint16_t* out;
-  const uint8_t* kc;
-  const uint8_t* vc;
-  const uint32_t* ks;
-  const uint32_t* vs;
-  const int32_t* bt;
-  const int32_t* ctxl;
-  float* ws;
-  uint32_t* cnt;
   int nchunk;
   Int4DecodeShape sh;
 };
 
-// A tile of the list: unit `u` (kv head * chunks + chunk) of sequence `seq`, tile t of n.
+// A tile of the list: tile t of the n of a unit (sequence, kv head, chunk of query heads).
 struct I4Tile {
-  int seq, u, t, n, ctx, ctx_next;
+  int seq, kvh, ch, t, n, ctx, ctx_next;
 };
 
 // float4s a lane keeps of a piece: [head tile][16-chunk tile][row r][half].
@@ -80,8 +72,8 @@ struct I4Geo {
 
 // The unit that a wave's first tile belongs to, where it was begun before the wave.
 struct I4Unit {
-  long long begin;   // its first tile in the list
-  int n, seq, u;
+  int begin;   // its first tile in the list
+  int n, seq, kvh, ch;
 };
 
 template <int STEPS, int HT>
@@ -90,10 +82,10 @@ struct alignas(16) I4Smem {
   f4_t acc[kI4Waves][G::NF][kWave];
   f2_t ml[kI4Waves][16 * HT];
   I4Unit head[kI4Waves];
-  int state[kI4Waves];
+  int state[kI4Waves], progress[kI4Waves];
   // the pieces of units that other work-groups share: [0] begun earlier, [1] continued later
   struct {
-    int active, first, count, seq, u, last;
+    int active, first, count, seq, kvh, ch, last;
   } piece[2];
   int last2;
 };
@@ -117,166 +109,276 @@ __device__ __forceinline__ void dev_store4(__amdgpu_buffer_rsrc_t r, int off, f4
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), r, off, 0, kPolicyDevice);
 }
 
+// Eight tokens' scores: lanes E0 .. E0 + 7 of a row hold their scale and minimum, which the
+// instructions read from there (a row broadcast each).  z = m qn + s c.  The compiler does not
+// see what is inside: the first half (E0 = 0) waits out the matrix instructions behind c and
+// the two states before a broadcast of values just written, the second comes after it.
+template <int E0>
+__device__ __forceinline__ void score8(float (&z)[16], float m, float s, float qn, const f4_t* c) {
+#define PA_MUL(K, E) "v_mul_f32_dpp %" #K ", %8, %10 row_newbcast:" #E " row_mask:0xf bank_mask:0xf\n\t"
+#define PA_FMAC(K, C, E) "v_fmac_f32_dpp %" #K ", %9, %" #C " row_newbcast:" #E " row_mask:0xf bank_mask:0xf\n\t"
+#define PA_OUT(E) "=&v"(z[E]), "=&v"(z[E + 1]), "=&v"(z[E + 2]), "=&v"(z[E + 3]), "=&v"(z[E + 4]), \
+                  "=&v"(z[E + 5]), "=&v"(z[E + 6]), "=&v"(z[E + 7])
+#define PA_IN(R) "v"(m), "v"(s), "v"(qn), "v"(c[0][R]), "v"(c[1][R]), "v"(c[2][R]), "v"(c[3][R]), \
+                 "v"(c[0][R + 1]), "v"(c[1][R + 1]), "v"(c[2][R + 1]), "v"(c[3][R + 1])
+  if constexpr (E0 == 0)
+    asm("s_nop 7\n\ts_nop 7\n\t" PA_MUL(0, 0) PA_MUL(1, 1) PA_MUL(2, 2) PA_MUL(3, 3) PA_MUL(4, 4) PA_MUL(5, 5)
+        PA_MUL(6, 6) PA_MUL(7, 7) PA_FMAC(0, 11, 0) PA_FMAC(1, 12, 1) PA_FMAC(2, 13, 2)
+        PA_FMAC(3, 14, 3) PA_FMAC(4, 15, 4) PA_FMAC(5, 16, 5) PA_FMAC(6, 17, 6) PA_FMAC(7, 18, 7)
+        : PA_OUT(0) : PA_IN(0));
+  else
+    asm(PA_MUL(0, 8) PA_MUL(1, 9) PA_MUL(2, 10) PA_MUL(3, 11) PA_MUL(4, 12)
+        PA_MUL(5, 13) PA_MUL(6, 14) PA_MUL(7, 15) PA_FMAC(0, 11, 8) PA_FMAC(1, 12, 9)
+        PA_FMAC(2, 13, 10) PA_FMAC(3, 14, 11) PA_FMAC(4, 15, 12) PA_FMAC(5, 16, 13)
+        PA_FMAC(6, 17, 14) PA_FMAC(7, 18, 15)
+        : PA_OUT(8) : PA_IN(2), "v"(z[0]));
+#undef PA_IN
+#undef PA_OUT
+#undef PA_FMAC
+#undef PA_MUL
+}
+// ... and their weights p: w = s p, B += m p.
+template <int E0>
+__device__ __forceinline__ void weight8(float (&w)[8], float& B, float m, float s,
+                                        const float (&p)[8]) {
+#define PA_MUL(K, P, E) "v_mul_f32_dpp %" #K ", %10, %" #P " row_newbcast:" #E " row_mask:0xf bank_mask:0xf\n\t"
+#define PA_FMAC(P, E) "v_fmac_f32_dpp %8, %9, %" #P " row_newbcast:" #E " row_mask:0xf bank_mask:0xf\n\t"
+#define PA_ARGS                                                                                 \
+  : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), \
+    "=&v"(w[7]), "+&v"(B) : "v"(m), "v"(s), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]),        \
+    "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7])
+  if constexpr (E0 == 0)
+    asm("s_nop 1\n\t" PA_MUL(0, 11, 0) PA_FMAC(11, 0) PA_MUL(1, 12, 1) PA_FMAC(12, 1)
+        PA_MUL(2, 13, 2) PA_FMAC(13, 2) PA_MUL(3, 14, 3) PA_FMAC(14, 3) PA_MUL(4, 15, 4)
+        PA_FMAC(15, 4) PA_MUL(5, 16, 5) PA_FMAC(16, 5) PA_MUL(6, 17, 6) PA_FMAC(17, 6)
+        PA_MUL(7, 18, 7) PA_FMAC(18, 7) PA_ARGS);
+  else
+    asm("s_nop 1\n\t" PA_MUL(0, 11, 8) PA_FMAC(11, 8) PA_MUL(1, 12, 9) PA_FMAC(12, 9)
+        PA_MUL(2, 13, 10) PA_FMAC(13, 10) PA_MUL(3, 14, 11) PA_FMAC(14, 11) PA_MUL(4, 15, 12)
+        PA_FMAC(15, 12) PA_MUL(5, 16, 13) PA_FMAC(16, 13) PA_MUL(6, 17, 14) PA_FMAC(17, 14)
+        PA_MUL(7, 18, 15) PA_FMAC(18, 15) PA_ARGS);
+#undef PA_ARGS
+#undef PA_FMAC
+#undef PA_MUL
+}
+// Max over the 16 lanes of a row.
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_mov<kQuadXor1>(v));
+  v = fmaxf(v, dpp_mov<kQuadXor2>(v));
+  v = fmaxf(v, dpp_mov<kRowHalfMirror>(v));
+  return fmaxf(v, dpp_mov<kRowMirror>(v));
+}
+__device__ __forceinline__ int select4(int a0, int a1, int a2, int a3, int k) {
+  const int lo = (k & 1) ? a1 : a0, hi = (k & 1) ? a3 : a2;
+  return (k & 2) ? hi : lo;
+}
+
 template <int STEPS, int HT, bool BF>
 __global__ void __launch_bounds__(kI4Waves* kWave) __attribute__((amdgpu_waves_per_eu(2)))
-decode_int4_kernel(I4Args a) {
+decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ ctxl, I4Args a,
+                   const uint16_t* __restrict__ q, const uint8_t* __restrict__ kc,
+                   const uint8_t* __restrict__ vc, const uint32_t* __restrict__ ks,
+                   const uint32_t* __restrict__ vs, uint16_t* __restrict__ out,
+                   float* __restrict__ ws, uint32_t* __restrict__ cnt) {
   using G = I4Geo<STEPS, HT>;
-  constexpr int T = G::T, NF = G::NF;
+  constexpr int T = G::T;
+  // the next unit's query is loaded a tile ahead where there are registers for it
+  constexpr bool kQueryAhead = STEPS * HT <= 4;
   __shared__ I4Smem<STEPS, HT> sm;
+  volatile int* prog = sm.progress;
   const Int4DecodeShape& sh = a.sh;
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int S = sh.num_seqs, U = sh.num_kv_heads * a.nchunk, C = sh.head_dim / 8, D = sh.head_dim;
   const int bs = 1 << sh.bs_log2;
   const int cap = sh.max_blocks << sh.bs_log2;
-  const size_t cell_bytes = (size_t)C * 4 << sh.bs_log2;   // bytes of a (block, head)
+  const uint32_t cell_bytes = (uint32_t)(C * 4) << sh.bs_log2;   // bytes of a (block, head)
 
-  // ---- the wave's range.  Lane l sums the tiles of sequences l per .. l per + per - 1.
+  // ---- the wave's range.  Lane l sums the tiles of sequences l per .. l per + per - 1 (all
+  // counts fit 31 bits: the host has checked the table's capacity).
   const int per = (S + kWave - 1) / kWave;
-  long long mine = 0;
+  uint32_t mine = 0;
+  int lane_ctx = 0;
   for (int j = 0; j < per; ++j) {
     const int s = lane * per + j;
-    if (s < S) mine += i4_tiles(i4_clamp_ctx(a.ctxl[s], cap));
+    lane_ctx = i4_clamp_ctx(ctxl[min(s, S - 1)], cap);
+    if (s < S) mine += i4_tiles(lane_ctx);
   }
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const long long y = __shfl_up(incl, o, kWave);
-    if (lane >= o) incl += y;
-  }
-  const long long W = __shfl(incl, kWave - 1, kWave) * U;
-  const long long want = (W + kI4Waves * kI4MinTiles - 1) / (kI4Waves * kI4MinTiles);
-  const int groups = want < kI4Groups ? (int)want : kI4Groups;
-  if ((int)blockIdx.x >= groups) return;
-  const long long N = (long long)groups * kI4Waves;
-  const long long widx = (long long)blockIdx.x * kI4Waves + wv;
-  const long long x0 = widx * W / N, x1 = (widx + 1) * W / N;
-  const int count = (int)(x1 - x0);
+  const uint32_t incl = wave_scan_dpp(mine);
+  const uint32_t W = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1) * (uint32_t)U;
+  const uint32_t want = (W + kI4Waves * kI4MinTiles - 1) / (kI4Waves * kI4MinTiles);
+  const uint32_t groups = want < kI4Groups ? want : kI4Groups;
+  const uint32_t b = blockIdx.x;
+  if (b >= groups) return;
+  // Work-group b takes W / groups tiles, the first W % groups one more; its waves likewise.
+  const uint32_t Q = W / groups, R = W - Q * groups;
+  const uint32_t gn = Q + (b < R ? 1u : 0u);
+  const uint32_t x0 = b * Q + min(b, R) + wv * (gn / kI4Waves) + min((uint32_t)wv, gn % kI4Waves);
+  const int count = (int)(gn / kI4Waves + ((uint32_t)wv < gn % kI4Waves ? 1u : 0u));
 
   I4Tile cur;
   {
-    // The sequence that holds x0: its lane by a ballot, then a walk over that lane's.
+    // The sequence that holds x0: its lane by a ballot, then, where a lane has several, a
+    // walk over that lane's.
     const unsigned long long before = __ballot(incl * U <= x0);
-    const int l = __builtin_popcountll(before);
-    long long base = l > 0 ? __shfl(incl, l - 1, kWave) : 0;
-    int s = l * per;
-    int ctx = 0, n = 1;
-    for (int j = 0; j < per; ++j) {
-      ctx = i4_clamp_ctx(a.ctxl[s < S ? s : S - 1], cap);
+    const int l = min((int)__builtin_popcountll(before), kWave - 1);
+    uint32_t base = l > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)incl, l - 1) : 0u;
+    int s = min(l * per, S - 1), n, ctx;
+    if (per == 1) {
+      ctx = __builtin_amdgcn_readlane(lane_ctx, s);
       n = i4_tiles(ctx);
-      if (s >= S - 1 || (base + n) * U > x0) break;
-      base += n;
-      ++s;
+      cur.ctx_next = __builtin_amdgcn_readlane(lane_ctx, min(s + 1, S - 1));
+    } else {
+      for (int j = 0;; ++j) {
+        ctx = i4_clamp_ctx(ctxl[s], cap);
+        n = i4_tiles(ctx);
+        if (j >= per - 1 || s >= S - 1 || (base + n) * U > x0) break;
+        base += n;
+        ++s;
+      }
+      cur.ctx_next = ctxl[min(s + 1, S - 1)];
     }
-    const long long in = x0 - base * U;
-    cur.seq = __builtin_amdgcn_readfirstlane(s < S ? s : S - 1);
-    cur.ctx = __builtin_amdgcn_readfirstlane(ctx);
-    cur.n = __builtin_amdgcn_readfirstlane(n);
-    cur.u = __builtin_amdgcn_readfirstlane((int)(in / n));
-    cur.t = __builtin_amdgcn_readfirstlane((int)(in % n));
-    cur.ctx_next = i4_clamp_ctx(a.ctxl[min(cur.seq + 1, S - 1)], cap);
+    const uint32_t in = x0 - base * U, u = in / (uint32_t)n;
+    cur.seq = s;
+    cur.ctx = ctx;
+    cur.n = n;
+    cur.t = (int)(in - u * n);
+    cur.kvh = (int)(u / (uint32_t)a.nchunk);
+    cur.ch = (int)u - cur.kvh * a.nchunk;
   }
 
   auto advance = [&](I4Tile& t) {
     if (++t.t < t.n) return;
     t.t = 0;
-    if (++t.u < U) return;
-    t.u = 0;
+    if (++t.ch < a.nchunk) return;
+    t.ch = 0;
+    if (++t.kvh < sh.num_kv_heads) return;
+    t.kvh = 0;
     t.seq = min(t.seq + 1, S - 1);
-    t.ctx = t.ctx_next;
+    t.ctx = i4_clamp_ctx(t.ctx_next, cap);
     t.n = i4_tiles(t.ctx);
-    t.ctx_next = i4_clamp_ctx(a.ctxl[min(t.seq + 1, S - 1)], cap);
+    t.ctx_next = ctxl[min(t.seq + 1, S - 1)];
   };
 
-  // ---- per-tile loads
+  // ---- per-tile loads.  The block ids of a tile's four 16-token groups, in scalar registers.
   struct Ids {
-    int k, v;
+    int b[4];
   };
-  auto load_ids = [&](const I4Tile& t) -> Ids {
-    Ids r{-1, -1};
+  auto load_ids = [&](const I4Tile& t) {
+    Ids r{{-1, -1, -1, -1}};
     if (t.ctx > 0) {
       const int lastb = (t.ctx - 1) >> sh.bs_log2;
-      const int32_t* row = a.bt + (size_t)t.seq * sh.max_blocks;
-      r.k = row[min((t.t * kI4Tile + 4 * i16) >> sh.bs_log2, lastb)];
-      r.v = row[min((t.t * kI4Tile + 16 * g) >> sh.bs_log2, lastb)];
+      const int32_t* row = bt + (size_t)t.seq * sh.max_blocks;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.b[j] = row[min((t.t * kI4Tile + 16 * j) >> sh.bs_log2, lastb)];
     }
     return r;
   };
-  auto safe = [&](int id) { return (uint32_t)id < (uint32_t)sh.num_blocks ? id : 0; };
-  uint4 kr[STEPS], vr[T][4], ksr[4], vsr[4];
-  const int k_last = min(4 * (STEPS - 1) + g, C - 1) * 16;
-  int v_chunk[T];
+  // The lane's block for K (tokens 4 i16 ..) and for V and the scales (16 g ..), 0 where the id
+  // is outside the pool, and how many of its 16 tokens exist (none then).
+  struct Where {
+    int k, v, live;
+  };
+  auto locate = [&](const I4Tile& t, const Ids& id) {
+    int sb[4], lv[4];
 #pragma unroll
-  for (int tt = 0; tt < T; ++tt) v_chunk[tt] = min(16 * tt + i16, C - 1) * 16;
-  auto load_k = [&](const I4Tile& t, int id) {
+    for (int j = 0; j < 4; ++j) {
+      const bool ok = (uint32_t)id.b[j] < (uint32_t)sh.num_blocks;
+      sb[j] = ok ? id.b[j] : 0;
+      lv[j] = ok ? t.ctx - (t.t * kI4Tile + 16 * j) : 0;
+    }
+    return Where{select4(sb[0], sb[1], sb[2], sb[3], i16 >> 2),
+                 select4(sb[0], sb[1], sb[2], sb[3], g), select4(lv[0], lv[1], lv[2], lv[3], g)};
+  };
+  uint4 kr[STEPS], vr[T][4];
+  uint32_t ksr, vsr;
+  // Byte offset of step j's 8 dims of K (of a query) for this lane.  Opaque to the compiler,
+  // which would otherwise keep each sum of such offsets in registers through the loop.
+  const uint32_t k_first = 16 * g, k_last = min(4 * (STEPS - 1) + g, C - 1) * 16;
+  auto k_chunk = [&](int j) {
+    uint32_t c = j < STEPS - 1 ? k_first : k_last;
+    asm volatile("" : "+v"(c));
+    return j < STEPS - 1 ? c + 64 * j : c;
+  };
+  const int v_step = C * 16;
+  auto load_k = [&](const I4Tile& t, const Where& w) {
     const int off = (t.t * kI4Tile + 4 * i16) & (bs - 1);
-    const uint8_t* p = a.kc + ((size_t)safe(id) * sh.num_kv_heads + t.u / a.nchunk) * cell_bytes +
-                       quad_offset(off, C);
+    const uint8_t* p = kc + (uint64_t)(uint32_t)(w.k * sh.num_kv_heads + t.kvh) * cell_bytes +
+                       (uint32_t)quad_offset(off, C);
 #pragma unroll
     for (int j = 0; j < STEPS; ++j)
-      kr[j] = *reinterpret_cast<const uint4*>(p + (j < STEPS - 1 ? 64 * j + 16 * g : k_last));
+      kr[j] = *reinterpret_cast<const uint4*>(p + k_chunk(j));
   };
-  auto load_scales = [&](const I4Tile& t, int id) {
-    const size_t bh = (size_t)safe(id) * sh.num_kv_heads + t.u / a.nchunk;
-    const size_t at = (bh << sh.bs_log2) + ((t.t * kI4Tile + 16 * g) & (bs - 1));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) ksr[j] = *reinterpret_cast<const uint4*>(a.ks + at + 4 * j);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vsr[j] = *reinterpret_cast<const uint4*>(a.vs + at + 4 * j);
+  // (lane (i, g) holds token 16 g + i's pairs; the rows broadcast them)
+  auto load_scales = [&](const I4Tile& t, const Where& w) {
+    const uint32_t bh = (uint32_t)(w.v * sh.num_kv_heads + t.kvh);
+    const uint64_t at = ((uint64_t)bh << sh.bs_log2) + ((t.t * kI4Tile + 16 * g) & (bs - 1)) + i16;
+    ksr = ks[at];
+    vsr = vs[at];
   };
-  auto load_v = [&](const I4Tile& t, int id) {
+  auto load_v = [&](const I4Tile& t, const Where& w) {
     const int off = (t.t * kI4Tile + 16 * g) & (bs - 1);
-    const uint8_t* p = a.vc + ((size_t)safe(id) * sh.num_kv_heads + t.u / a.nchunk) * cell_bytes +
-                       quad_offset(off, C);
+    const uint8_t* p = vc + (uint64_t)(uint32_t)(w.v * sh.num_kv_heads + t.kvh) * cell_bytes +
+                       (uint32_t)quad_offset(off, C);
 #pragma unroll
-    for (int tt = 0; tt < T; ++tt)
+    for (int tt = 0; tt < T; ++tt) {
+      uint32_t c = min(16 * tt + i16, C - 1) * 16;
+      asm volatile("" : "+v"(c));
+      const uint8_t* row = p + c;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        vr[tt][k] = *reinterpret_cast<const uint4*>(p + k * C * 16 + v_chunk[tt]);
+      for (int k = 0; k < 4; ++k) {
+        vr[tt][k] = load_stream<uint4>(row);
+        row += v_step;
+      }
+    }
   };
 
-  // ---- the query of a unit: raw rows, then the matrix operand and its two factors
-  uint4 qr[HT][STEPS];
-  float cs[HT], qs[HT];
+  // ---- the query of a unit: raw rows, then the matrix operand.  Scores in its units: those
+  // of base 2 are cs z, cs >= 0 (a negative scale turns the query round).
+  uint4 qr[HT][STEPS], qa[HT][STEPS];
+  float cs[HT], qn[HT];
   auto load_q = [&](const I4Tile& t) {
-    const int kvh = t.u / a.nchunk, ch = t.u - kvh * a.nchunk;
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      const int hh = min(ch * 16 * HT + ht * 16 + i16, sh.group - 1);
-      const uint16_t* row = a.q + ((size_t)t.seq * sh.num_heads + kvh * sh.group + hh) * D;
+      const int hh = min(t.ch * 16 * HT + ht * 16 + i16, sh.group - 1);
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(
+          q + ((size_t)t.seq * sh.num_heads + t.kvh * sh.group + hh) * D);
 #pragma unroll
       for (int j = 0; j < STEPS; ++j)
-        qr[ht][j] = *reinterpret_cast<const uint4*>(row + min(4 * j + g, C - 1) * 8);
+        qa[ht][j] = *reinterpret_cast<const uint4*>(row + k_chunk(j));
     }
   };
   auto convert_q = [&]() {
+    const float sgn = sh.scale_log2 < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
       float mx = 0.f, sum = 0.f;
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        if (4 * j + g >= C) qr[ht][j] = make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {qr[ht][j].x, qr[ht][j].y, qr[ht][j].z, qr[ht][j].w};
+        if (4 * j + g >= C) qa[ht][j] = make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {qa[ht][j].x, qa[ht][j].y, qa[ht][j].z, qa[ht][j].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float lo = widen_lo<BF>(w[k]), hi = widen_hi<BF>(w[k]);
           mx = fmaxf(mx, fmaxf(fabsf(lo), fabsf(hi)));
           sum += lo + hi;
         }
+        // (the second pass widens the rows again, as there are no registers to keep them wide)
+        asm volatile("" : "+v"(qa[ht][j].x), "+v"(qa[ht][j].y), "+v"(qa[ht][j].z), "+v"(qa[ht][j].w));
       }
       mx = head_max(mx);
       sum = head_sum(sum);
       const int e = 15 - __builtin_amdgcn_frexp_expf(mx);   // |q| 2^e < 2^15
-      cs[ht] = __builtin_amdgcn_ldexpf(sh.scale_log2 * kCode24, -e);
-      qs[ht] = sh.scale_log2 * sum;
+      cs[ht] = __builtin_amdgcn_ldexpf(fabsf(sh.scale_log2), 24 - e);
+      qn[ht] = __builtin_amdgcn_ldexpf(sgn * sum, e - 24);
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        const uint32_t w[4] = {qr[ht][j].x, qr[ht][j].y, qr[ht][j].z, qr[ht][j].w};
+        const uint32_t w[4] = {qa[ht][j].x, qa[ht][j].y, qa[ht][j].z, qa[ht][j].w};
         float x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          x[2 * k] = __builtin_amdgcn_ldexpf(widen_lo<BF>(w[k]), e);
-          x[2 * k + 1] = __builtin_amdgcn_ldexpf(widen_hi<BF>(w[k]), e - 4);
+          x[2 * k] = __builtin_amdgcn_ldexpf(sgn * widen_lo<BF>(w[k]), e);
+          x[2 * k + 1] = __builtin_amdgcn_ldexpf(sgn * widen_hi<BF>(w[k]), e - 4);
         }
         qr[ht][j] = make_uint4(pack_h2(x[0], x[4]), pack_h2(x[1], x[5]), pack_h2(x[2], x[6]),
                                pack_h2(x[3], x[7]));
@@ -299,8 +401,9 @@ decode_int4_kernel(I4Args a) {
     }
   };
 
-  auto process = [&](const I4Tile& t, int idv, bool more, const I4Tile& nx, Ids idn) {
-    // scores of the codes
+  // One tile, its rows in registers; MORE: the next one's loads go out as registers fall free.
+  auto process = [&](auto MORE, int live, const I4Tile& nx, const Where& wn) {
+    constexpr bool kMore = decltype(MORE)::value;
     f4_t sc[HT][4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -315,41 +418,41 @@ decode_int4_kernel(I4Args a) {
           sc[ht][n] = mfma16(ka, __builtin_bit_cast(h8_t, qr[ht][j]), sc[ht][n]);
       }
     }
-    if (more) {
-      if (nx.t == 0) load_q(nx);
-      load_k(nx, idn.k);
+    if constexpr (kMore) {
+      if (!kQueryAhead && nx.t == 0) load_q(nx);
+      load_k(nx, wn);
     }
-    // tokens of the lane's 16 that exist
-    int live = t.ctx - (t.t * kI4Tile + 16 * g);
-    if ((uint32_t)idv >= (uint32_t)sh.num_blocks) live = 0;
-    uint32_t kw[16], vw[16];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      kw[4 * k] = ksr[k].x, kw[4 * k + 1] = ksr[k].y, kw[4 * k + 2] = ksr[k].z, kw[4 * k + 3] = ksr[k].w;
-      vw[4 * k] = vsr[k].x, vw[4 * k + 1] = vsr[k].y, vw[4 * k + 2] = vsr[k].z, vw[4 * k + 3] = vsr[k].w;
-    }
+    // the lane's own token's scales; nothing of a token that does not exist
+    const bool mine_live = i16 < live;
+    const uint32_t kp = mine_live ? ksr : 0u, vp = mine_live ? vsr : 0u;
+    const float s_k = widen_lo<false>(kp), m_k = widen_hi<false>(kp);
+    const float s_v = widen_lo<false>(vp), m_v = widen_hi<false>(vp);
+    if constexpr (kMore) load_scales(nx, wn);
+    // (2^-24: fp16's smallest step, for rows of one value, whose scale is 0)
+    const float log_s = __builtin_amdgcn_logf(fmaxf(row_max(s_v), 0x1p-24f));
     const bool full = __all(live >= 16);
-    if (!full) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e >= live) kw[e] = vw[e] = 0;
-    }
     h8_t phi[HT][2], plo[HT][2];
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      float z[16], mx = M[ht];
+      float z[16];
+      score8<0>(z, m_k, s_k, qn[ht], sc[ht]);
+      score8<8>(z, m_k, s_k, qn[ht], sc[ht]);
+      if (!full) {
+        asm volatile("");   // (a branch: most tiles are full)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const half2_t k2 = __builtin_bit_cast(half2_t, kw[e]), v2 = __builtin_bit_cast(half2_t, vw[e]);
-        z[e] = __builtin_fmaf((float)k2.x, sc[ht][e & 3][e >> 2] * cs[ht], (float)k2.y * qs[ht]);
-        if (!full && e >= live) z[e] = kNegInf;
-        // (2^-24: fp16's smallest step, for rows of one value, whose scale is 0)
-        mx = fmaxf(mx, z[e] + __builtin_amdgcn_logf(fmaxf((float)v2.x, 0x1p-24f)));
+        for (int e = 0; e < 16; ++e) z[e] = e < live ? z[e] : kNegInf;
       }
+      float mx = fmaxf(z[0], z[1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
+      // (a tile without tokens: -inf, also where cs is 0)
+      mx = mx == kNegInf ? kNegInf : __builtin_fmaf(mx, cs[ht], log_s);
       mx = head_max(mx);
-      const float f = M[ht] == kNegInf ? 0.f : exp2f_fast(M[ht] - mx);
-      const float ref = mx == kNegInf ? 0.f : mx - kShift;
-      if (__any(mx != M[ht])) {
+      // The reference moves when it is passed by kSlack: the weights then stay below 2^16.
+      const bool move = mx > M[ht] + kSlack;
+      if (__any(move)) {
+        const float f = !move ? 1.f : (M[ht] == kNegInf ? 0.f : exp2f_fast(M[ht] - mx));
+        M[ht] = move ? mx : M[ht];
 #pragma unroll
         for (int tt = 0; tt < T; ++tt)
 #pragma unroll
@@ -357,20 +460,29 @@ decode_int4_kernel(I4Args a) {
         L[ht] *= f;
         B[ht] *= f;
       }
-      M[ht] = mx;
+      const float ref = M[ht] == kNegInf ? 0.f : M[ht] - kShift;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const half2_t v2 = __builtin_bit_cast(half2_t, vw[e]);
-        const float p = exp2f_fast(z[e] - ref);
-        L[ht] += p;
-        B[ht] = __builtin_fmaf(p, (float)v2.y, B[ht]);
-        const float ps = p * (float)v2.x;
-        const half_t hi = (half_t)ps;
-        phi[ht][e >> 3][e & 7] = hi;
-        plo[ht][e >> 3][e & 7] = (half_t)(ps - (float)hi);
+      for (int hf = 0; hf < 2; ++hf) {
+        float p[8], w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = exp2f_fast(__builtin_fmaf(z[8 * hf + e], cs[ht], -ref));
+          L[ht] += p[e];
+        }
+        if (hf == 0) weight8<0>(w, B[ht], m_v, s_v, p);
+        else weight8<8>(w, B[ht], m_v, s_v, p);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          // (towards zero: the second number holds what that leaves)
+          const auto hi = __builtin_amdgcn_cvt_pkrtz(w[e], w[e + 1]);
+          const auto lo = __builtin_amdgcn_cvt_pkrtz(w[e] - (float)hi[0], w[e + 1] - (float)hi[1]);
+          phi[ht][hf][e] = hi[0];
+          phi[ht][hf][e + 1] = hi[1];
+          plo[ht][hf][e] = lo[0];
+          plo[ht][hf][e + 1] = lo[1];
+        }
       }
     }
-    if (more) load_scales(nx, idn.v);
     // weighted codes
 #pragma unroll
     for (int tt = 0; tt < T; ++tt) {
@@ -380,15 +492,16 @@ decode_int4_kernel(I4Args a) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t sel = half ? 0x07060302u : 0x05040100u;
-          u4_t w = {__builtin_amdgcn_perm(a0.y, a0.x, sel), __builtin_amdgcn_perm(a0.w, a0.z, sel),
-                    __builtin_amdgcn_perm(a1.y, a1.x, sel), __builtin_amdgcn_perm(a1.w, a1.z, sel)};
+          const u4_t w = {
+              __builtin_amdgcn_perm(a0.y, a0.x, sel), __builtin_amdgcn_perm(a0.w, a0.z, sel),
+              __builtin_amdgcn_perm(a1.y, a1.x, sel), __builtin_amdgcn_perm(a1.w, a1.z, sel)};
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            if (b == 2) w = w >> 8;
-            const h8_t va = __builtin_bit_cast(h8_t, w & ((b & 1) ? 0x00F000F0u : 0x000F000Fu));
+          for (int d = 0; d < 4; ++d) {
+            const u4_t x = d < 2 ? w << 2 : w >> 6;
+            const h8_t va = __builtin_bit_cast(h8_t, x & ((d & 1) ? 0x03C003C0u : 0x003C003Cu));
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
-              f4_t& o = acc[ht][tt][4 * half + b];
+              f4_t& o = acc[ht][tt][4 * half + d];
               o = mfma16(va, phi[ht][hf], o);
               o = mfma16(va, plo[ht][hf], o);
             }
@@ -396,7 +509,7 @@ decode_int4_kernel(I4Args a) {
         }
       }
     }
-    if (more) load_v(nx, idn.v);
+    if constexpr (kMore) load_v(nx, wn);
   };
 
   // The state as a piece: sums over the head's lanes, outputs in their own units.
@@ -412,31 +525,32 @@ decode_int4_kernel(I4Args a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             acc[ht][tt][n][r] =
-                __builtin_fmaf(acc[ht][tt][n][r], (n & 1) ? kCode24 / 16.f : kCode24, B[ht]);
+                __builtin_fmaf(acc[ht][tt][n][r], (n & 1) ? kCode24 / 64.f : kCode24 / 4.f, B[ht]);
     }
   };
   auto piece4 = [&](int ht, int tt, int r, int half) {
     return (f4_t){acc[ht][tt][4 * half][r], acc[ht][tt][4 * half + 1][r],
                   acc[ht][tt][4 * half + 2][r], acc[ht][tt][4 * half + 3][r]};
   };
-  auto write_out = [&](int seq, int u) {
-    const int kvh = u / a.nchunk, ch = u - kvh * a.nchunk;
+  auto write_out = [&](int seq, int kvh, int ch) {
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
       const int hh = ch * 16 * HT + ht * 16 + i16;
       const float inv = L[ht] != 0.f ? 1.f / L[ht] : 0.f;
+      int gq = g;
+      asm volatile("" : "+v"(gq));   // (as k_chunk)
 #pragma unroll
       for (int tt = 0; tt < T; ++tt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int chunk = 16 * tt + 4 * g + r;
+          const int chunk = 16 * tt + 4 * gq + r;
           if (hh >= sh.group || chunk >= C) continue;
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             w[k] = pack2<BF>(acc[ht][tt][2 * k][r] * inv, acc[ht][tt][2 * k + 1][r] * inv);
           *reinterpret_cast<uint4*>(
-              a.out + ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D + chunk * 8) =
+              out + ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D + chunk * 8) =
               make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
@@ -448,104 +562,138 @@ decode_int4_kernel(I4Args a) {
   if (count > 0) {
     if (t0 != 0) {
       state |= kHead;
-      if (lane == 0) sm.head[wv] = I4Unit{x0 - t0, cur.n, cur.seq, cur.u};
+      if (lane == 0) sm.head[wv] = I4Unit{(int)x0 - t0, cur.n, cur.seq, cur.kvh, cur.ch};
     }
-    reset();
-    Ids id = load_ids(cur);
-    load_q(cur);
-    load_k(cur, id.k);
-    load_scales(cur, id.v);
-    load_v(cur, id.v);
     I4Tile nx = cur;
-    Ids idn{-1, -1};
+    Where w = locate(cur, load_ids(cur));
+    load_q(cur);
+    load_k(cur, w);
+    load_scales(cur, w);
+    load_v(cur, w);
+    int live = w.live;
+    Ids idn{{-1, -1, -1, -1}};
     if (count > 1) {
       advance(nx);
       idn = load_ids(nx);
     }
-    bool fresh = true;
-    for (int k = 0; k < count; ++k) {
-      const bool more = k + 1 < count;
-      if (fresh) convert_q();
+    prog[wv] = 0;
+    reset();
+    convert_q();
+    if (kQueryAhead && count > 1 && nx.t == 0) load_q(nx);
+    // What a unit's last tile, or the wave's, leaves to be done.
+    auto finish = [&](bool ends, bool head) {
+      to_piece();
+      if (head) {
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+          for (int tt = 0; tt < T; ++tt)
+#pragma unroll
+            for (int f = 0; f < 8; ++f)
+              sm.acc[wv][(ht * T + tt) * 8 + f][lane] = piece4(ht, tt, f >> 1, f & 1);
+          if (g == 0) sm.ml[wv][ht * 16 + i16] = (f2_t){M[ht], L[ht]};
+        }
+        if (ends) state |= kHeadEnds;
+      } else if (ends) {
+        write_out(cur.seq, cur.kvh, cur.ch);
+      } else {
+        state |= kTail;
+      }
+    };
+    // (head: the unit was begun before the wave, whose tiles it still holds without a break)
+    for (int k = 0; k < count - 1; ++k) {
+      // Of the SIMD's two waves the one behind goes first (left alone, the older does).
+      const int other = __builtin_amdgcn_readfirstlane(prog[wv ^ 4]);
+      if (k <= other) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+      prog[wv] = k + 1;
+      w = locate(nx, idn);
       I4Tile nn = nx;
-      Ids id2{-1, -1};
       if (k + 2 < count) {
         advance(nn);
-        id2 = load_ids(nn);
+        idn = load_ids(nn);
       }
-      process(cur, id.v, more, nx, idn);
-      fresh = cur.t == cur.n - 1;                       // the unit ends here
-      const bool head = (state & kHead) && cur.t == t0 + k;   // ... and was begun before the wave
-      if (fresh || !more) {
-        to_piece();
-        if (head) {
-#pragma unroll
-          for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-            for (int tt = 0; tt < T; ++tt)
-#pragma unroll
-              for (int f = 0; f < 8; ++f)
-                sm.acc[wv][(ht * T + tt) * 8 + f][lane] = piece4(ht, tt, f >> 1, f & 1);
-            if (g == 0) sm.ml[wv][ht * 16 + i16] = (f2_t){M[ht], L[ht]};
-          }
-          if (fresh) state |= kHeadEnds;
-        } else if (fresh) {
-          write_out(cur.seq, cur.u);
-        } else {
-          state |= kTail;
-        }
-        if (more) reset();
+      process(std::true_type(), live, nx, w);
+      if (nx.t == 0) {
+        finish(true, (state & kHead) && cur.t == t0 + k);
+        reset();
+        convert_q();
       }
-      if (more) {
-        cur = nx;
-        id = idn;
-        nx = nn;
-        idn = id2;
-      }
+      live = w.live;
+      cur = nx;
+      nx = nn;
+      if (kQueryAhead && k + 2 < count && nx.t == 0) load_q(nx);
     }
+    process(std::false_type(), live, nx, w);
+    finish(cur.t == cur.n - 1, (state & kHead) && cur.t == t0 + count - 1);
   }
   if (lane == 0) sm.state[wv] = state;
   if (threadIdx.x < 2) sm.piece[threadIdx.x].active = 0;
   __syncthreads();
 
   // ---- units that several waves share.  The wave that began one folds the waves' behind it.
-  auto fold_slot = [&](int w) {
+  // Folds the slots of waves w, w + 1, .. until the unit ends, K of them at most; the reads of
+  // all are under way together (unused ones read the first again, weighted 0).
+  auto fold_slots = [&](auto KC, const int (&slot)[4], int n) __attribute__((always_inline)) {
+    constexpr int K = decltype(KC)::value;
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      const f2_t ml = sm.ml[w][ht * 16 + i16];
-      const float mx = fmaxf(M[ht], ml.x);
-      const float f1 = M[ht] == kNegInf ? 0.f : exp2f_fast(M[ht] - mx);
-      const float f2 = ml.x == kNegInf ? 0.f : exp2f_fast(ml.x - mx);
+      f2_t ml[K];
+      float mx = M[ht], f[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        ml[k] = sm.ml[slot[k]][ht * 16 + i16];
+        mx = fmaxf(mx, ml[k].x);
+      }
+      const float own = M[ht] == kNegInf ? 0.f : exp2f_fast(M[ht] - mx);
       M[ht] = mx;
-      L[ht] = L[ht] * f1 + ml.y * f2;
+      L[ht] *= own;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        f[k] = k >= n || ml[k].x == kNegInf ? 0.f : exp2f_fast(ml[k].x - mx);
+        L[ht] = __builtin_fmaf(ml[k].y, f[k], L[ht]);
+      }
 #pragma unroll
       for (int tt = 0; tt < T; ++tt)
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
-          const f4_t v = sm.acc[w][(ht * T + tt) * 8 + f][lane];
+        for (int i = 0; i < 8; ++i) {
+          f4_t s;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f4_t& o = acc[ht][tt][4 * (f & 1) + k];
-            o[f >> 1] = o[f >> 1] * f1 + v[k] * f2;
-          }
+          for (int e = 0; e < 4; ++e) s[e] = acc[ht][tt][4 * (i & 1) + e][i >> 1] * own;
+#pragma unroll
+          for (int k = 0; k < K; ++k) s += sm.acc[slot[k]][(ht * T + tt) * 8 + i][lane] * f[k];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[ht][tt][4 * (i & 1) + e][i >> 1] = s[e];
         }
     }
   };
-  // Folds the slots of waves w, w + 1, ..; whether the unit ends among them.
-  auto fold_from = [&](int w) {
-    for (; w < kI4Waves; ++w) {
-      const int st = __builtin_amdgcn_readfirstlane(sm.state[w]);
-      if (!(st & kHasTiles)) continue;
-      fold_slot(w);
-      if (st & kHeadEnds) return true;
+  // ... and whether it does.
+  auto fold_from = [&](int w) __attribute__((always_inline)) {
+    bool ended = false;
+    while (w < kI4Waves && !ended) {
+      int slot[4], n = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) slot[k] = 0;
+      for (; w < kI4Waves && n < 4 && !ended; ++w) {
+        const int st = __builtin_amdgcn_readfirstlane(sm.state[w]);
+        if (!(st & kHasTiles)) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) slot[k] = k >= n ? w : slot[k];
+        ++n;
+        ended = (st & kHeadEnds) != 0;
+      }
+      if (n == 1) fold_slots(std::integral_constant<int, 1>(), slot, n);
+      else if (n > 1) fold_slots(std::integral_constant<int, 4>(), slot, n);
     }
-    return false;
+    return ended;
   };
-  auto worker_group = [&](long long x) {          // the work-group whose range holds tile x
-    return (int)((((x + 1) * N - 1) / W) / kI4Waves);
+  auto worker_group = [&](uint32_t x) {          // the work-group whose range holds tile x
+    const uint32_t big = R * (Q + 1);
+    return (int)(x < big ? x / (Q + 1) : R + (x - big) / Q);
   };
   // The piece of a unit that other work-groups share: into memory, to be counted below.
-  auto share = [&](int which, long long begin, int n, int seq, int u) {
-    float* slot = a.ws + (size_t)(2 * blockIdx.x + which) * G::kSlotFloats;
+  auto share = [&](int which, const I4Unit& u) {
+    float* slot = ws + (size_t)(2 * b + which) * G::kSlotFloats;
     const auto rs = buf_rsrc(slot, (uint32_t)(G::kSlotFloats * 4));
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
@@ -564,15 +712,16 @@ decode_int4_kernel(I4Args a) {
     if (lane == 0) {
       auto& p = sm.piece[which];
       p.active = 1;
-      p.first = worker_group(begin);
-      p.count = worker_group(begin + n - 1) - p.first + 1;
-      p.seq = seq;
-      p.u = u;
+      p.first = worker_group(u.begin);
+      p.count = worker_group(u.begin + u.n - 1) - p.first + 1;
+      p.seq = u.seq;
+      p.kvh = u.kvh;
+      p.ch = u.ch;
     }
   };
   if (state & kTail) {
-    if (fold_from(wv + 1)) write_out(cur.seq, cur.u);
-    else share(1, x1 - 1 - cur.t, cur.n, cur.seq, cur.u);
+    if (fold_from(wv + 1)) write_out(cur.seq, cur.kvh, cur.ch);
+    else share(1, I4Unit{(int)x0 + count - 1 - cur.t, cur.n, cur.seq, cur.kvh, cur.ch});
   }
   if (wv == 0) {
     int w = 0;
@@ -581,7 +730,7 @@ decode_int4_kernel(I4Args a) {
     if (w < kI4Waves && (sm.state[w] & kHead)) {
       reset();
       fold_from(w);
-      share(0, sm.head[w].begin, sm.head[w].n, sm.head[w].seq, sm.head[w].u);
+      share(0, sm.head[w]);
     }
   }
   // ---- units that several work-groups share: the last to arrive merges the pieces.
@@ -589,7 +738,6 @@ decode_int4_kernel(I4Args a) {
   __builtin_amdgcn_s_waitcnt(0);
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __syncthreads();
-  const int b = blockIdx.x;
   auto arrive = [&](uint32_t* c, int n) {
     const bool last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                       (uint32_t)(n - 1);
@@ -602,18 +750,19 @@ decode_int4_kernel(I4Args a) {
     if (p.active) {
       // groups of kMergeMax consecutive pieces; the first group's counter is the first
       // work-group's own, which no other unit has, a later group's its first member's
-      const int gi = (b - p.first) / kMergeMax, m0 = p.first + gi * kMergeMax;
-      p.last = arrive(a.cnt + (gi == 0 ? 0 : kI4Groups) + m0, min(kMergeMax, p.first + p.count - m0));
+      const int gi = ((int)b - p.first) / kMergeMax, m0 = p.first + gi * kMergeMax;
+      p.last = arrive(cnt + (gi == 0 ? 0 : kI4Groups) + m0, min(kMergeMax, p.first + p.count - m0));
     }
   }
   __syncthreads();
   // Merges n pieces, those of work-groups m0, m0 + step, ..: the output, or one piece in
   // place of the first.
-  auto merge = [&](int first, int m0, int step, int n, bool final_out, int seq, int u) {
-    const int kvh = u / a.nchunk, ch = u - kvh * a.nchunk;
+  auto merge_of = [&](auto KC, int first, int m0, int step, int n, bool final_out, int seq, int kvh,
+                      int ch) __attribute__((always_inline)) {
+    constexpr int K = decltype(KC)::value;
     auto slot_of = [&](int j) {
       const int m = m0 + j * step;
-      return a.ws + (size_t)(2 * m + (m == first ? 1 : 0)) * G::kSlotFloats;
+      return ws + (size_t)(2 * m + (m == first ? 1 : 0)) * G::kSlotFloats;
     };
     f4_t A[T * HT];
     float Mi[T * HT], Li[T * HT];
@@ -621,26 +770,28 @@ decode_int4_kernel(I4Args a) {
     for (int q = 0; q < T * HT; ++q) {
       const int f = wv + q * kI4Waves;                  // (ht * T + tt) * 8 + 2 r + half
       const int h = (f / (8 * T)) * 16 + i16;
-      f4_t v[kMergeMax];
-      f2_t ml[kMergeMax];
-#pragma unroll
-      for (int j = 0; j < kMergeMax; ++j) {
-        // (past the last piece it is read again and weighted 0: every load is unconditional)
-        const auto rs = buf_rsrc(slot_of(min(j, n - 1)), (uint32_t)(G::kSlotFloats * 4));
-        v[j] = dev_load4(rs, (f * kWave + lane) * 16);
-        ml[j] = __builtin_bit_cast(f2_t, __builtin_amdgcn_raw_buffer_load_b64(
-                                             rs, G::kPieceFloats * 4 + h * 8, 0, kPolicyDevice));
-      }
-      float mx = kNegInf;
-#pragma unroll
-      for (int j = 0; j < kMergeMax; ++j)
-        if (j < n) mx = fmaxf(mx, ml[j].x);
+      float mx = kNegInf, l = 0.f;
       f4_t s = {0.f, 0.f, 0.f, 0.f};
-      float l = 0.f;
+      for (int j0 = 0; j0 < n; j0 += K) {
+        f4_t v[K];
+        f2_t ml[K];
 #pragma unroll
-      for (int j = 0; j < kMergeMax; ++j) {
-        const float w = j >= n || ml[j].x == kNegInf ? 0.f : exp2f_fast(ml[j].x - mx);
-        if (j < n) {
+        for (int j = 0; j < K; ++j) {
+          // (past the last piece it is read again and weighted 0: every load is unconditional)
+          const auto rs = buf_rsrc(slot_of(min(j0 + j, n - 1)), (uint32_t)(G::kSlotFloats * 4));
+          v[j] = dev_load4(rs, (f * kWave + lane) * 16);
+          ml[j] = __builtin_bit_cast(f2_t, __builtin_amdgcn_raw_buffer_load_b64(
+                                               rs, G::kPieceFloats * 4 + h * 8, 0, kPolicyDevice));
+        }
+        const float old = mx;
+#pragma unroll
+        for (int j = 0; j < K; ++j) mx = fmaxf(mx, ml[j].x);
+        const float keep = old == kNegInf ? 0.f : exp2f_fast(old - mx);
+        s *= keep;
+        l *= keep;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          const float w = j0 + j >= n || ml[j].x == kNegInf ? 0.f : exp2f_fast(ml[j].x - mx);
           s += v[j] * w;
           l += ml[j].y * w;
         }
@@ -659,7 +810,7 @@ decode_int4_kernel(I4Args a) {
         const float inv = Li[q] != 0.f ? 1.f / Li[q] : 0.f;
         const uint2 w = make_uint2(pack2<BF>(A[q][0] * inv, A[q][1] * inv),
                                    pack2<BF>(A[q][2] * inv, A[q][3] * inv));
-        *reinterpret_cast<uint2*>(a.out +
+        *reinterpret_cast<uint2*>(out +
                                   ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D +
                                   chunk * 8 + 4 * (f & 1)) = w;
       }
@@ -681,27 +832,35 @@ decode_int4_kernel(I4Args a) {
       }
     }
   };
+  auto merge = [&](int first, int m0, int step, int n, bool final_out, int seq, int kvh,
+                   int ch) __attribute__((always_inline)) {
+    if (n <= 4)
+      merge_of(std::integral_constant<int, 4>(), first, m0, step, n, final_out, seq, kvh, ch);
+    else
+      merge_of(std::integral_constant<int, 8>(), first, m0, step, n, final_out, seq, kvh, ch);
+  };
   for (int which = 0; which < 2; ++which) {
     const auto p = sm.piece[which];
     if (!__builtin_amdgcn_readfirstlane(p.last)) continue;
     const int first = __builtin_amdgcn_readfirstlane(p.first);
     const int np = __builtin_amdgcn_readfirstlane(p.count);
-    const int seq = __builtin_amdgcn_readfirstlane(p.seq), u = __builtin_amdgcn_readfirstlane(p.u);
-    const int gi = (b - first) / kMergeMax, m0 = first + gi * kMergeMax;
+    const int seq = __builtin_amdgcn_readfirstlane(p.seq);
+    const int kvh = __builtin_amdgcn_readfirstlane(p.kvh), ch = __builtin_amdgcn_readfirstlane(p.ch);
+    const int gi = ((int)b - first) / kMergeMax, m0 = first + gi * kMergeMax;
     const int n = min(kMergeMax, first + np - m0);
     if (np <= kMergeMax) {
-      merge(first, m0, 1, n, true, seq, u);
+      merge(first, m0, 1, n, true, seq, kvh, ch);
       continue;
     }
-    merge(first, m0, 1, n, false, seq, u);
+    merge(first, m0, 1, n, false, seq, kvh, ch);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_waitcnt(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __syncthreads();
     const int ng = (np + kMergeMax - 1) / kMergeMax;
-    if (threadIdx.x == 0) sm.last2 = arrive(a.cnt + 2 * kI4Groups + first, ng);
+    if (threadIdx.x == 0) sm.last2 = arrive(cnt + 2 * kI4Groups + first, ng);
     __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(sm.last2)) merge(first, first, kMergeMax, ng, true, seq, u);
+    if (__builtin_amdgcn_readfirstlane(sm.last2)) merge(first, first, kMergeMax, ng, true, seq, kvh, ch);
     __syncthreads();   // (last2 is written again by the other piece)
   }
 }
@@ -710,12 +869,12 @@ namespace {
 
 template <int HT, bool BF>
 hipError_t launch_tiles(const Int4Decode& l) {
-  I4Args a{static_cast<const uint16_t*>(l.q), static_cast<uint16_t*>(l.out),
-           static_cast<const uint8_t*>(l.k_cache), static_cast<const uint8_t*>(l.v_cache),
-           static_cast<const uint32_t*>(l.k_scales), static_cast<const uint32_t*>(l.v_scales),
-           l.block_table, l.context_lens, l.workspace, l.counters,
-           (l.shape.group + 16 * HT - 1) / (16 * HT), l.shape};
-  decode_int4_kernel<PA_INT4_STEPS, HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(a);
+  const I4Args a{(l.shape.group + 16 * HT - 1) / (16 * HT), l.shape};
+  decode_int4_kernel<PA_INT4_STEPS, HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
+      l.block_table, l.context_lens, a, static_cast<const uint16_t*>(l.q),
+      static_cast<const uint8_t*>(l.k_cache), static_cast<const uint8_t*>(l.v_cache),
+      static_cast<const uint32_t*>(l.k_scales), static_cast<const uint32_t*>(l.v_scales),
+      static_cast<uint16_t*>(l.out), l.workspace, l.counters);
   return hipGetLastError();
 }
 
