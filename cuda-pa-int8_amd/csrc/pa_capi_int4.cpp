@@ -17,7 +17,8 @@ pa_status_t check_cache(int32_t head_dim, int32_t num_kv_heads, int32_t num_bloc
   if (block_size <= 0 || block_size % 16 != 0 || 128 % block_size != 0)
     return PA_ERR_BAD_BLOCK_SIZE;
   if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0) return PA_ERR_UNSUPPORTED;
-  if (num_kv_heads < 1 || num_blocks < 1) return PA_ERR_BAD_SHAPE;
+  if (num_kv_heads < 1 || num_blocks < 1 || (int64_t)num_blocks * num_kv_heads > UINT32_MAX)
+    return PA_ERR_BAD_SHAPE;
   return PA_OK;
 }
 
@@ -53,8 +54,7 @@ pa_status_t decode_shape(int32_t num_seqs, int32_t num_heads, int32_t head_dim,
   const pa_status_t st = check_cache(head_dim, num_kv_heads, num_blocks, block_size);
   if (st != PA_OK) return st;
   if (num_seqs < 0 || num_heads < 1 || num_heads % num_kv_heads != 0 || max_blocks < 0 ||
-      (int64_t)max_blocks * block_size > INT32_MAX - 128 ||
-      (int64_t)num_blocks * num_kv_heads > UINT32_MAX)
+      (int64_t)max_blocks * block_size > INT32_MAX - 128)
     return PA_ERR_BAD_SHAPE;
   // The kernel counts 64-token tiles of every (sequence, query head) in 31 bits.
   const int64_t tiles = (int64_t)max_blocks * block_size / 64 + 1;
