@@ -6,18 +6,24 @@
 //   row cu_s + i: position ctx_s + i, slot table[s][position / bs] * bs + position % bs
 //
 // One launch.  Every work-group scans the batch's lengths itself (a few KB from the
-// caches) and keeps the prefix sums in LDS; the token rows and the new table entries are then
-// dealt to all of them, each finding its sequence by a search in LDS.  A new block's id
-// comes straight from the free list, so no work-group reads what another writes.  The
-// lengths and the free count may be updated in place: the work-group that arrives
-// last, when all others have read them, writes both.  What bounds it is latency: the launch,
-// two dependent loads, the scan and the stores.
-#include "pa_int4.hpp"
+// caches).  Where no sequence gets more than kFew tokens (decode steps) the first one's
+// threads place their own sequences' rows; else the prefix sums are kept in LDS and the token
+// rows are dealt to all work-groups, each thread finding its sequence by a search there; a
+// new block's first row enters it in the table.  A new block's id comes straight from the free
+// list, so no work-group reads what another writes.  The lengths and the free count may be updated in place:
+// the work-group that arrives last, when all others have read them, writes both.
+//
+// What bounds it is latency: the launch, two dependent loads, the scan and the stores.
+// MI355X, replayed from a graph: one token for each of 256 sequences 3.1 us (6.1 with 1024
+// threads, the searches and 64-bit shuffles of a first version), 64 prompts of 98,575 tokens 3.9
+// (7.3), in place 6.8.
+#include "pa_decode_kernels.hpp"
 
 namespace pa {
 
-constexpr int kExtThreads = 1024;
+constexpr int kExtThreads = 256;
 constexpr int kExtPer = kExtendMaxSeqs / kExtThreads;   // sequences of one thread, at most
+constexpr int kFew = 4;
 
 struct ExtendArgs {
   int32_t* bt;
@@ -27,6 +33,7 @@ struct ExtendArgs {
   int32_t *cu, *status;
   uint32_t* counter;
   int seqs, max_blocks, bs_log2, rows, free_cap;
+  bool in_place;
 };
 
 // The largest index i < n with pre[i] <= x (pre ascending, pre[0] = 0 <= x); of equal
@@ -41,138 +48,162 @@ __device__ __forceinline__ int last_at_most(const int* pre, int n, int x) {
   return lo;
 }
 
+// Inclusive prefix sum over the wave of counts below 2^31, in 64 bits.
+__device__ __forceinline__ long long wave_scan64(uint32_t v) {
+  return ((long long)wave_scan_dpp(v >> 16) << 16) + wave_scan_dpp(v & 0xFFFFu);
+}
+
+template <int PER>
 __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
+  constexpr int NW = kExtThreads / kWave;
   extern __shared__ int lds[];               // cu, first, ctx of each sequence
-  __shared__ long long wsum[2][kExtThreads / kWave];
-  __shared__ int flags;
+  __shared__ long long wsum[2][NW];
+  __shared__ int wflag[NW];
   __shared__ bool last;
   const int S = a.seqs, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid >> 6;
-  int *cu = lds, *first = lds + S, *ctx = lds + 2 * S;
-  const int per = (S + kExtThreads - 1) / kExtThreads, s0 = tid * per;
-  const int bs = 1 << a.bs_log2;
-  if (tid == 0) flags = 0;
+  const int s0 = tid * PER, bs = 1 << a.bs_log2;
   const int nfree = *a.num_free;
-  int n[kExtPer], need[kExtPer];
-  long long tn = 0, tb = 0;
-  int bad = 0;
+  int c[PER], n[PER], need[PER];
 #pragma unroll
-  for (int i = 0; i < kExtPer; ++i) {
-    n[i] = need[i] = 0;
-    const int s = s0 + i;
-    if (i < per && s < S) {
-      const int c = a.ctx[s], w = a.nw[s];
-      ctx[s] = c;
-      if (c < 0 || w < 0) {
-        bad |= kExtendBadLength;
-      } else {
-        const long long have = ((long long)c + bs - 1) >> a.bs_log2;
-        const long long want = ((long long)c + w + bs - 1) >> a.bs_log2;
-        if (want > a.max_blocks || (long long)c + w > INT32_MAX) bad |= kExtendRowFull;
-        n[i] = w;
-        need[i] = (int)(want - have);
-        tn += w;
-        tb += want - have;
-      }
-    }
+  for (int i = 0; i < PER; ++i) {
+    const int s = min(s0 + i, S - 1);
+    c[i] = a.ctx[s];
+    n[i] = a.nw[s];
   }
-  // Exclusive scan over the threads: a wave's lanes by shuffles, the waves through LDS.
-  long long xn = tn, xb = tb;
+  int bad = 0;
+  bool many = false;
+  long long xn = 0, xb = 0;   // inclusive sums up to this thread, within the wave
 #pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const long long yn = __shfl_up(xn, o, kWave), yb = __shfl_up(xb, o, kWave);
-    if (lane >= o) {
-      xn += yn;
-      xb += yb;
+  for (int i = 0; i < PER; ++i) {
+    need[i] = 0;
+    if (s0 + i >= S || c[i] < 0 || n[i] < 0) {
+      if (s0 + i < S) bad |= kExtendBadLength;
+      n[i] = 0;
+    } else {
+      const long long have = ((long long)c[i] + bs - 1) >> a.bs_log2;
+      const long long want = ((long long)c[i] + n[i] + bs - 1) >> a.bs_log2;
+      if (want > a.max_blocks || (long long)c[i] + n[i] > INT32_MAX) bad |= kExtendRowFull;
+      need[i] = (int)(want - have);
+      many |= n[i] > kFew;
     }
+    xn += wave_scan64((uint32_t)n[i]);      // (a sum over i of scans is the scan of the sums)
+    xb += wave_scan64((uint32_t)need[i]);
   }
   if (lane == kWave - 1) {
     wsum[0][wv] = xn;
     wsum[1][wv] = xb;
   }
+  // one bit for each reason, and one for a long row of new tokens
+  const int f1 = __any(bad & kExtendBadLength) ? kExtendBadLength : 0;
+  const int f2 = __any(bad & kExtendRowFull) ? kExtendRowFull : 0;
+  const int f3 = __any(many) ? 16 : 0;
+  if (lane == 0) wflag[wv] = f1 | f2 | f3;
   __syncthreads();
   long long alln = 0, allb = 0;
-  for (int w = 0; w < kExtThreads / kWave; ++w) {
-    if (w == wv) {
-      xn += alln;
-      xb += allb;
+  int st = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < wv) {
+      xn += wsum[0][w];
+      xb += wsum[1][w];
     }
     alln += wsum[0][w];
     allb += wsum[1][w];
+    st |= wflag[w];
   }
-  if (nfree < 0 || nfree > a.free_cap) bad |= kExtendBadLength;
-  else if (allb > nfree) bad |= kExtendNoBlocks;
-  if (alln > a.rows) bad |= kExtendNoRows;
-  if (bad) atomicOr(&flags, bad);
-  long long en = xn - tn, eb = xb - tb;
-#pragma unroll
-  for (int i = 0; i < kExtPer; ++i) {
-    const int s = s0 + i;
-    if (i < per && s < S) {
-      cu[s] = (int)en;
-      first[s] = (int)eb;
-      en += n[i];
-      eb += need[i];
-    }
-  }
-  __syncthreads();
-  const int st = flags;
+  // (counted now, looked at in the end)
+  uint32_t arrived = 0;
+  if (tid == 0 && gridDim.x > 1 && a.in_place)
+    arrived = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const bool search = (st & 16) != 0;
+  st &= 15;
+  if (nfree < 0 || nfree > a.free_cap) st |= kExtendBadLength;
+  else if (allb > nfree) st |= kExtendNoBlocks;
+  if (alln > a.rows) st |= kExtendNoRows;
   const int live = st ? 0 : (int)alln, blocks = st ? 0 : (int)allb;
+#pragma unroll
+  for (int i = PER - 1; i >= 0; --i) {       // exclusive, from the thread's last sequence down
+    xn -= n[i];
+    xb -= need[i];
+    if (search && s0 + i < S) {
+      lds[s0 + i] = (int)xn;
+      lds[S + s0 + i] = (int)xb;
+      lds[2 * S + s0 + i] = c[i];
+    }
+    if (blockIdx.x == 0 && s0 + i < S) {
+      if (a.cu) a.cu[s0 + i] = st ? 0 : (int)xn;
+      if (!search && !st) {
+        const int have = (c[i] + bs - 1) >> a.bs_log2;
+        int32_t* row = a.bt + (size_t)(s0 + i) * a.max_blocks;
+        for (int k = 0; k < n[i]; ++k) {
+          const int p = c[i] + k, b = (p >> a.bs_log2) - have;
+          const int blk = b < 0 ? row[p >> a.bs_log2] : a.free[nfree - 1 - ((int)xb + b)];
+          if (b >= 0 && (p & (bs - 1)) == 0) row[p >> a.bs_log2] = blk;
+          a.slots[(int)xn + k] = (int64_t)blk * bs + (p & (bs - 1));
+          if (a.pos) a.pos[(int)xn + k] = p;
+        }
+      }
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    if (a.cu) a.cu[S] = live;
+    *a.status = st;
+  }
   const int stride = gridDim.x * kExtThreads;
-  // New table entries, then the rows.
-  for (int e = blockIdx.x * kExtThreads + tid; e < blocks; e += stride) {
-    const int s = last_at_most(first, S, e);
-    const int have = (ctx[s] + bs - 1) >> a.bs_log2;
-    a.bt[(size_t)s * a.max_blocks + have + (e - first[s])] = a.free[nfree - 1 - e];
-  }
-  for (int r = blockIdx.x * kExtThreads + tid; r < a.rows; r += stride) {
-    int64_t slot = -1, p = 0;
-    if (r < live) {
+  int r = blockIdx.x * kExtThreads + tid;
+  if (search) {
+    __syncthreads();
+    const int *cu = lds, *first = lds + S, *ctx = lds + 2 * S;
+    for (; r < live; r += stride) {
       const int s = last_at_most(cu, S, r);
-      const int c = ctx[s], pos = c + (r - cu[s]);
-      const int j = (pos >> a.bs_log2) - ((c + bs - 1) >> a.bs_log2);
-      const int blk = j < 0 ? a.bt[(size_t)s * a.max_blocks + (pos >> a.bs_log2)]
-                            : a.free[nfree - 1 - (first[s] + j)];
-      slot = (int64_t)blk * bs + (pos & (bs - 1));
-      p = pos;
+      const int c0 = ctx[s], p = c0 + (r - cu[s]);
+      const int b = (p >> a.bs_log2) - ((c0 + bs - 1) >> a.bs_log2);
+      int32_t* entry = a.bt + (size_t)s * a.max_blocks + (p >> a.bs_log2);
+      const int blk = b < 0 ? *entry : a.free[nfree - 1 - (first[s] + b)];
+      if (b >= 0 && (p & (bs - 1)) == 0) *entry = blk;    // (a new block's first token)
+      a.slots[r] = (int64_t)blk * bs + (p & (bs - 1));
+      if (a.pos) a.pos[r] = p;
     }
-    a.slots[r] = slot;
-    if (a.pos) a.pos[r] = p;
   }
-  if (blockIdx.x == 0) {
-    if (a.cu) {
-      for (int s = tid; s < S; s += kExtThreads) a.cu[s] = st ? 0 : cu[s];
-      if (tid == 0) a.cu[S] = live;
+  // Rows behind the last token.
+  for (; r < a.rows; r += stride)
+    if (r >= live) {
+      a.slots[r] = -1;
+      if (a.pos) a.pos[r] = 0;
     }
-    if (tid == 0) *a.status = st;
-  }
-  // In-place outputs: by the last arrival, with every work-group's reads behind it (their
-  // values have been used, in the scan above).
-  if (gridDim.x > 1) {
-    if (tid == 0)
-      last = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-             gridDim.x - 1;
+  // The new lengths: by the first work-group; in place, when every one has read the old ones
+  // (its waves before the barrier above), by the last to arrive.
+  if (!a.in_place) {
+    if (blockIdx.x != 0) return;
+  } else if (gridDim.x > 1) {
+    if (tid == 0) last = arrived == gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     if (tid == 0) *a.counter = 0;
   }
 #pragma unroll
-  for (int i = 0; i < kExtPer; ++i) {
-    const int s = s0 + i;
-    if (i < per && s < S) a.ctx_out[s] = ctx[s] + (st ? 0 : n[i]);
-  }
+  for (int i = 0; i < PER; ++i)
+    if (s0 + i < S) a.ctx_out[s0 + i] = c[i] + (st ? 0 : n[i]);
   if (tid == 0) *a.num_free_out = nfree - blocks;
 }
 
 hipError_t launch_extend(const ExtendLaunch& l) {
+  auto overlap = [&](const int32_t* x, const int32_t* y, int n) { return x < y + n && y < x + n; };
+  const bool in_place = overlap(l.context_lens_out, l.context_lens, l.num_seqs) ||
+                        overlap(l.num_free_out, l.num_free, 1);
   ExtendArgs a{l.block_table, l.context_lens, l.new_lens, l.free_blocks, l.num_free,
                l.context_lens_out, l.num_free_out, l.slot_mapping, l.positions, l.cu_seqlens,
                l.status, l.counter, l.num_seqs, l.max_blocks,
-               __builtin_ctz((unsigned)l.block_size), l.num_rows, l.free_capacity};
-  // (two rows a thread; the scan, repeated by each work-group, is what more of them cost)
-  int grid = (l.num_rows + 2 * kExtThreads - 1) / (2 * kExtThreads);
-  grid = grid < 1 ? 1 : (grid > 256 ? 256 : grid);
-  extend_kernel<<<grid, kExtThreads, 3 * sizeof(int) * (l.num_seqs > 0 ? l.num_seqs : 1),
-                  l.stream>>>(a);
+               __builtin_ctz((unsigned)l.block_size), l.num_rows, l.free_capacity, in_place};
+  // One row a thread; in place fewer work-groups, as their arrivals are counted in one word,
+  // one after another (98,575 rows: 64 work-groups 8.3 us, 256 6.8).
+  const int most = in_place ? 256 : 512;
+  int grid = (l.num_rows + kExtThreads - 1) / kExtThreads;
+  grid = grid < 1 ? 1 : (grid > most ? most : grid);
+  const size_t lds = 3 * sizeof(int) * l.num_seqs;
+  const int per = (l.num_seqs + kExtThreads - 1) / kExtThreads;
+  auto* k = per <= 1 ? extend_kernel<1> : (per <= 4 ? extend_kernel<4> : extend_kernel<kExtPer>);
+  k<<<grid, kExtThreads, lds, l.stream>>>(a);
   return hipGetLastError();
 }
 
