@@ -72,7 +72,7 @@ struct I4Geo {
 
 // The unit that a wave's first tile belongs to, where it was begun before the wave.
 struct I4Unit {
-  int begin;   // its first tile in the list
+  uint32_t begin;   // its start in the list
   int n, seq, kvh, ch;
 };
 
@@ -81,7 +81,7 @@ struct alignas(16) I4Smem {
   using G = I4Geo<STEPS, HT>;
   f4_t acc[kI4Waves][G::NF][kWave];
   f2_t ml[kI4Waves][16 * HT];
-  I4Unit head[kI4Waves];
+  I4Unit head[kI4Waves], tail[kI4Waves];
   int state[kI4Waves], progress[kI4Waves];
   // the pieces of units that other work-groups share: [0] begun earlier, [1] continued later
   struct {
@@ -182,6 +182,10 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
                    float* __restrict__ ws, uint32_t* __restrict__ cnt) {
   using G = I4Geo<STEPS, HT>;
   constexpr int T = G::T;
+  // The waves' pieces of one unit are folded by all of them where a piece is one float4 a thread
+  // (32 x 4096 at 12/2 heads 15.7 -> 14.9 us; with two, slower than by their first wave: 64
+  // ragged sequences at 32/1 24.6 against 26.4).
+  constexpr bool kTogether = T * HT == 1;
   // the next unit's query is loaded a tile ahead where there are registers for it
   constexpr bool kQueryAhead = STEPS * HT <= 4;
   __shared__ I4Smem<STEPS, HT> sm;
@@ -197,55 +201,80 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
   // ---- the wave's range.  Lane l sums the tiles of sequences l per .. l per + per - 1 (all
   // counts fit 31 bits: the host has checked the table's capacity).
   const int per = (S + kWave - 1) / kWave;
-  uint32_t mine = 0;
+  uint32_t mine = 0, shortest = ~0u, longest = 0;
   int lane_ctx = 0;
   for (int j = 0; j < per; ++j) {
     const int s = lane * per + j;
     lane_ctx = i4_clamp_ctx(ctxl[min(s, S - 1)], cap);
-    if (s < S) mine += i4_tiles(lane_ctx);
+    const uint32_t n = i4_tiles(lane_ctx);
+    mine += s < S ? n : 0u;
+    shortest = min(shortest, n);
+    longest = max(longest, n);
   }
   const uint32_t incl = wave_scan_dpp(mine);
-  const uint32_t W = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1) * (uint32_t)U;
-  const uint32_t want = (W + kI4Waves * kI4MinTiles - 1) / (kI4Waves * kI4MinTiles);
+  const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1) * (uint32_t)U;
+  // The list is divided by cost: 2 for a tile and 1 for a unit's start and end, where the units
+  // differ and a wave has tiles enough to make up for it; else evenly by tiles, as equal
+  // units divide best.
+  const uint32_t first_n = (uint32_t)__builtin_amdgcn_readfirstlane((int)shortest);
+  const bool ragged = __any(shortest != first_n || longest != first_n);
+  const bool weigh = ragged && tiles >= 4u * kI4Groups * kI4Waves;
+  const uint32_t tile_cost = weigh ? 2u : 1u, unit_cost = weigh ? 1u : 0u;
+  const uint32_t W = tiles * tile_cost + (uint32_t)(S * U) * unit_cost;
+  const uint32_t want = (tiles + kI4Waves * kI4MinTiles - 1) / (kI4Waves * kI4MinTiles);
   const uint32_t groups = want < kI4Groups ? want : kI4Groups;
   const uint32_t b = blockIdx.x;
   if (b >= groups) return;
-  // Work-group b takes W / groups tiles, the first W % groups one more; its waves likewise.
+  // Work-group b takes W / groups of the cost, the first W % groups one more; its waves
+  // likewise.  A point of the list at cost x stands for the tile there (a unit's first, at
+  // its start).
   const uint32_t Q = W / groups, R = W - Q * groups;
   const uint32_t gn = Q + (b < R ? 1u : 0u);
   const uint32_t x0 = b * Q + min(b, R) + wv * (gn / kI4Waves) + min((uint32_t)wv, gn % kI4Waves);
-  const int count = (int)(gn / kI4Waves + ((uint32_t)wv < gn % kI4Waves ? 1u : 0u));
+  const uint32_t x1 = x0 + gn / kI4Waves + ((uint32_t)wv < gn % kI4Waves ? 1u : 0u);
 
-  I4Tile cur;
-  {
-    // The sequence that holds x0: its lane by a ballot, then, where a lane has several, a
-    // walk over that lane's.
-    const unsigned long long before = __ballot(incl * U <= x0);
+  // The tile at cost x < W (where its unit starts, in `begin`), and its index in the list.
+  const uint32_t lane_seqs = (uint32_t)min((lane + 1) * per, S);
+  const uint32_t lane_cost = (incl * tile_cost + lane_seqs * unit_cost) * (uint32_t)U;
+  auto tile_at = [&](uint32_t x, I4Tile& t, uint32_t& begin) {
+    // The sequence: its lane by a ballot, then, where a lane has several, a walk over that
+    // lane's.
+    const unsigned long long before = __ballot(lane_cost <= x);
     const int l = min((int)__builtin_popcountll(before), kWave - 1);
     uint32_t base = l > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)incl, l - 1) : 0u;
     int s = min(l * per, S - 1), n, ctx;
     if (per == 1) {
       ctx = __builtin_amdgcn_readlane(lane_ctx, s);
       n = i4_tiles(ctx);
-      cur.ctx_next = __builtin_amdgcn_readlane(lane_ctx, min(s + 1, S - 1));
+      t.ctx_next = __builtin_amdgcn_readlane(lane_ctx, min(s + 1, S - 1));
     } else {
       for (int j = 0;; ++j) {
         ctx = i4_clamp_ctx(ctxl[s], cap);
         n = i4_tiles(ctx);
-        if (j >= per - 1 || s >= S - 1 || (base + n) * U > x0) break;
+        if (j >= per - 1 || s >= S - 1 ||
+            ((base + n) * tile_cost + (uint32_t)(s + 1) * unit_cost) * U > x)
+          break;
         base += n;
         ++s;
       }
-      cur.ctx_next = ctxl[min(s + 1, S - 1)];
+      t.ctx_next = ctxl[min(s + 1, S - 1)];
     }
-    const uint32_t in = x0 - base * U, u = in / (uint32_t)n;
-    cur.seq = s;
-    cur.ctx = ctx;
-    cur.n = n;
-    cur.t = (int)(in - u * n);
-    cur.kvh = (int)(u / (uint32_t)a.nchunk);
-    cur.ch = (int)u - cur.kvh * a.nchunk;
-  }
+    const uint32_t unit = (uint32_t)n * tile_cost + unit_cost;
+    const uint32_t in = x - (base * tile_cost + (uint32_t)s * unit_cost) * U, u = in / unit;
+    const uint32_t c = in - u * unit;
+    begin = x - c;
+    t.seq = s;
+    t.ctx = ctx;
+    t.n = n;
+    t.t = c < unit_cost ? 0 : (int)((c - unit_cost) / tile_cost);
+    t.kvh = (int)(u / (uint32_t)a.nchunk);
+    t.ch = (int)u - t.kvh * a.nchunk;
+    return base * U + u * n + (uint32_t)t.t;
+  };
+  I4Tile cur, after;
+  uint32_t unit0, unit1 = W;     // where the units at both ends of the range start
+  const uint32_t tile0 = tile_at(x0, cur, unit0);
+  const int count = (int)((x1 < W ? tile_at(x1, after, unit1) : tiles) - tile0);
 
   auto advance = [&](I4Tile& t) {
     if (++t.t < t.n) return;
@@ -562,7 +591,7 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
   if (count > 0) {
     if (t0 != 0) {
       state |= kHead;
-      if (lane == 0) sm.head[wv] = I4Unit{(int)x0 - t0, cur.n, cur.seq, cur.kvh, cur.ch};
+      if (lane == 0) sm.head[wv] = I4Unit{unit0, cur.n, cur.seq, cur.kvh, cur.ch};
     }
     I4Tile nx = cur;
     Where w = locate(cur, load_ids(cur));
@@ -580,19 +609,22 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
     reset();
     convert_q();
     if (kQueryAhead && count > 1 && nx.t == 0) load_q(nx);
+    auto to_slot = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+        for (int tt = 0; tt < T; ++tt)
+#pragma unroll
+          for (int f = 0; f < 8; ++f)
+            sm.acc[wv][(ht * T + tt) * 8 + f][lane] = piece4(ht, tt, f >> 1, f & 1);
+        if (g == 0) sm.ml[wv][ht * 16 + i16] = (f2_t){M[ht], L[ht]};
+      }
+    };
     // What a unit's last tile, or the wave's, leaves to be done.
     auto finish = [&](bool ends, bool head) {
       to_piece();
       if (head) {
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-          for (int tt = 0; tt < T; ++tt)
-#pragma unroll
-            for (int f = 0; f < 8; ++f)
-              sm.acc[wv][(ht * T + tt) * 8 + f][lane] = piece4(ht, tt, f >> 1, f & 1);
-          if (g == 0) sm.ml[wv][ht * 16 + i16] = (f2_t){M[ht], L[ht]};
-        }
+        to_slot();
         if (ends) state |= kHeadEnds;
       } else if (ends) {
         write_out(cur.seq, cur.kvh, cur.ch);
@@ -626,14 +658,34 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
     }
     process(std::false_type(), live, nx, w);
     finish(cur.t == cur.n - 1, (state & kHead) && cur.t == t0 + count - 1);
+    if (kTogether && (state & (kHead | kTail)) == kTail) {
+      to_slot();
+      if (lane == 0) sm.tail[wv] = I4Unit{unit1, cur.n, cur.seq, cur.kvh, cur.ch};
+    }
   }
   if (lane == 0) sm.state[wv] = state;
   if (threadIdx.x < 2) sm.piece[threadIdx.x].active = 0;
   __syncthreads();
 
+  // What the waves have, a bit each.
+  const int st_lane = sm.state[lane & (kI4Waves - 1)];
+  auto waves_with = [&](int bit) {
+    return (uint32_t)__ballot(lane < kI4Waves && (st_lane & bit) != 0);
+  };
+  const uint32_t w_tiles = waves_with(kHasTiles), w_head = waves_with(kHead);
+  const uint32_t w_ends = waves_with(kHeadEnds), w_tail = waves_with(kTail);
+  // The waves with pieces of the unit that wave w has the first of, up to its end; and whether
+  // it ends among them.
+  auto behind_of = [&](int w, bool from_head, bool& ended) {
+    const uint32_t later = from_head ? ~0u << w : ~0u << (w + 1);
+    const uint32_t end = w_ends & later;
+    ended = end != 0;
+    return w_tiles & later & (ended ? (end ^ (end - 1)) : ~0u);   // up to the lowest end
+  };
+
   // ---- units that several waves share.  The wave that began one folds the waves' behind it.
-  // Folds the slots of waves w, w + 1, .. until the unit ends, K of them at most; the reads of
-  // all are under way together (unused ones read the first again, weighted 0).
+  // Folds the slots of n waves, K at most, into the wave's own state; the reads of all are
+  // under way together (unused ones read the first again, weighted 0).
   auto fold_slots = [&](auto KC, const int (&slot)[4], int n) __attribute__((always_inline)) {
     constexpr int K = decltype(KC)::value;
 #pragma unroll
@@ -667,32 +719,29 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
         }
     }
   };
-  // ... and whether it does.
-  auto fold_from = [&](int w) __attribute__((always_inline)) {
-    bool ended = false;
-    while (w < kI4Waves && !ended) {
+  auto fold_waves = [&](uint32_t members) __attribute__((always_inline)) {
+    while (members != 0) {
       int slot[4], n = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) slot[k] = 0;
-      for (; w < kI4Waves && n < 4 && !ended; ++w) {
-        const int st = __builtin_amdgcn_readfirstlane(sm.state[w]);
-        if (!(st & kHasTiles)) continue;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) slot[k] = k >= n ? w : slot[k];
-        ++n;
-        ended = (st & kHeadEnds) != 0;
+      for (int k = 0; k < 4; ++k) {
+        if (members != 0) {
+          slot[k] = __builtin_ctz(members);
+          members &= members - 1;
+          n = k + 1;
+        } else {
+          slot[k] = slot[0];
+        }
       }
       if (n == 1) fold_slots(std::integral_constant<int, 1>(), slot, n);
-      else if (n > 1) fold_slots(std::integral_constant<int, 4>(), slot, n);
+      else fold_slots(std::integral_constant<int, 4>(), slot, n);
     }
-    return ended;
   };
-  auto worker_group = [&](uint32_t x) {          // the work-group whose range holds tile x
+  auto worker_group = [&](uint32_t x) {          // the last work-group that starts at x or before
     const uint32_t big = R * (Q + 1);
     return (int)(x < big ? x / (Q + 1) : R + (x - big) / Q);
   };
   // The piece of a unit that other work-groups share: into memory, to be counted below.
-  auto share = [&](int which, const I4Unit& u) {
+  auto share = [&](int which) {
     float* slot = ws + (size_t)(2 * b + which) * G::kSlotFloats;
     const auto rs = buf_rsrc(slot, (uint32_t)(G::kSlotFloats * 4));
 #pragma unroll
@@ -709,28 +758,92 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
                                               kPolicyDevice);
       }
     }
-    if (lane == 0) {
-      auto& p = sm.piece[which];
-      p.active = 1;
-      p.first = worker_group(u.begin);
-      p.count = worker_group(u.begin + u.n - 1) - p.first + 1;
-      p.seq = u.seq;
-      p.kvh = u.kvh;
-      p.ch = u.ch;
-    }
   };
-  if (state & kTail) {
-    if (fold_from(wv + 1)) write_out(cur.seq, cur.kvh, cur.ch);
-    else share(1, I4Unit{(int)x0 + count - 1 - cur.t, cur.n, cur.seq, cur.kvh, cur.ch});
-  }
-  if (wv == 0) {
-    int w = 0;
-    while (w < kI4Waves && !(sm.state[w] & kHasTiles)) ++w;
-    w = __builtin_amdgcn_readfirstlane(w);
-    if (w < kI4Waves && (sm.state[w] & kHead)) {
+  // Four dims of a head (item f of a piece) as outputs.
+  auto store_item = [&](int seq, int kvh, int ch, int f, f4_t s, float l) {
+    const int hh = ch * 16 * HT + (f / (8 * T)) * 16 + i16;
+    const int chunk = ((f / 8) % T) * 16 + 4 * g + ((f & 7) >> 1);
+    if (hh >= sh.group || chunk >= C) return;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<uint2*>(out + ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D +
+                              chunk * 8 + 4 * (f & 1)) =
+        make_uint2(pack2<BF>(s[0] * inv, s[1] * inv), pack2<BF>(s[2] * inv, s[3] * inv));
+  };
+  auto note_shared = [&](int which, const I4Unit& u) {
+    auto& p = sm.piece[which];
+    p.active = 1;
+    // (the points that stand for the unit's first tile, and all of the unit's)
+    p.first = worker_group(u.begin + unit_cost + tile_cost - 1);
+    p.count = worker_group(u.begin + unit_cost + u.n * tile_cost - 1) - p.first + 1;
+    p.seq = u.seq;
+    p.kvh = u.kvh;
+    p.ch = u.ch;
+  };
+  // A unit's first piece here: one begun, or the first wave's, of a unit begun before.
+  const uint32_t lead = w_head & (w_tiles & (0u - w_tiles)), starts = w_tail | lead;
+  if (kTogether && (w_head & w_tail) == 0 && (starts & (starts - 1)) == 0) {
+    // One unit at most, and every wave's piece of it in its slot: all waves fold them
+    // together, four dims of a head per lane.
+    if (starts != 0) {
+      const int w0 = __builtin_ctz(starts);
+      const bool begun = w_tail != 0;
+      bool ended;
+      const uint32_t members = behind_of(w0, !begun, ended) | starts;
+      const I4Unit unit = begun ? sm.tail[w0] : sm.head[w0];
+      const int which = begun ? 1 : 0;
+#pragma unroll
+      for (int q2 = 0; q2 < T * HT; ++q2) {
+        const int f = wv + q2 * kI4Waves, h = (f / (8 * T)) * 16 + i16;
+        f2_t ml[kI4Waves];
+        f4_t v[kI4Waves];
+        float mx = kNegInf, l = 0.f;
+#pragma unroll
+        for (int k = 0; k < kI4Waves; ++k) {
+          const int src = ((members >> k) & 1) ? k : w0;
+          ml[k] = sm.ml[src][h];
+          v[k] = sm.acc[src][f][lane];
+          mx = fmaxf(mx, ml[k].x);
+        }
+        f4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kI4Waves; ++k) {
+          const float e = !((members >> k) & 1) || ml[k].x == kNegInf ? 0.f : exp2f_fast(ml[k].x - mx);
+          s += v[k] * e;
+          l += ml[k].y * e;
+        }
+        if (begun && ended) {
+          store_item(unit.seq, unit.kvh, unit.ch, f, s, l);
+        } else {
+          const auto rs = buf_rsrc(ws + (size_t)(2 * b + which) * G::kSlotFloats,
+                                   (uint32_t)(G::kSlotFloats * 4));
+          dev_store4(rs, (f * kWave + lane) * 16, s);
+          if (f % (8 * T) == 0 && g == 0) {
+            const f2_t p = {mx, l};
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2_t, p), rs,
+                                                  G::kPieceFloats * 4 + h * 8, 0, kPolicyDevice);
+          }
+        }
+      }
+      if (!(begun && ended) && threadIdx.x == 0) note_shared(which, unit);
+    }
+  } else {
+    bool ended;
+    if (state & kTail) {
+      const uint32_t behind = behind_of(wv, false, ended);
+      fold_waves(behind);
+      if (ended) {
+        write_out(cur.seq, cur.kvh, cur.ch);
+      } else {
+        share(1);
+        if (lane == 0) note_shared(1, I4Unit{unit1, cur.n, cur.seq, cur.kvh, cur.ch});
+      }
+    }
+    if (wv == 0 && lead != 0) {
+      const int w = __builtin_ctz(lead);
       reset();
-      fold_from(w);
-      share(0, sm.head[w]);
+      fold_waves(behind_of(w, true, ended));
+      share(0);
+      if (lane == 0) note_shared(0, sm.head[w]);
     }
   }
   // ---- units that several work-groups share: the last to arrive merges the pieces.
@@ -802,18 +915,8 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
     }
     if (final_out) {
 #pragma unroll
-      for (int q = 0; q < T * HT; ++q) {
-        const int f = wv + q * kI4Waves;
-        const int hh = ch * 16 * HT + (f / (8 * T)) * 16 + i16;
-        const int chunk = ((f / 8) % T) * 16 + 4 * g + ((f & 7) >> 1);
-        if (hh >= sh.group || chunk >= C) continue;
-        const float inv = Li[q] != 0.f ? 1.f / Li[q] : 0.f;
-        const uint2 w = make_uint2(pack2<BF>(A[q][0] * inv, A[q][1] * inv),
-                                   pack2<BF>(A[q][2] * inv, A[q][3] * inv));
-        *reinterpret_cast<uint2*>(out +
-                                  ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D +
-                                  chunk * 8 + 4 * (f & 1)) = w;
-      }
+      for (int q = 0; q < T * HT; ++q)
+        store_item(seq, kvh, ch, wv + q * kI4Waves, A[q], Li[q]);
     } else {
       // (each thread rewrites the items that it alone read; the pairs, which all read, after
       // a barrier)
