@@ -27,6 +27,8 @@ step appended to the cache and answered by the split-K decode kernel over it
   length live on the device; ``generate_greedy_graph`` replays it per token.
   The eager loop's time per token is the host launching 28 layers' kernels;
   the replay's is the device's.
+* A ``PagedKVCache`` of 4 bits takes its prompt in as many chunks as one likes: a further
+  chunk attends to the cached values of those before it.
 * Every model call computes the logits of its last position only
   (``logits_to_keep=1``): a 1024-token prompt's full logits would be 0.3 GB.
 """
@@ -99,7 +101,10 @@ class DecodeSession:
         self.position = 0
         self._token = None
         self._graph = None         # the DecodeGraph being warmed up or captured
-        if getattr(cache, "is_int8", False):
+        self._int4 = getattr(cache, "is_int4", False)
+        if self._int4:
+            self._kernel = "int4"
+        elif getattr(cache, "is_int8", False):
             self._kernel = "splitk_int8"
         else:
             self._kernel = "splitk"
@@ -140,6 +145,8 @@ class DecodeSession:
         if n > 1:
             if self._graph is not None:
                 raise RuntimeError("a captured decode step feeds one token")
+            if self._int4 and c.lengths[layer] > 0:
+                return self._attend_chunk(layer, query, key, value, scaling)
             c.prefill(layer, k_tok.contiguous(), v_tok.contiguous())
             return _prefill_attention(query, key, value, scaling).transpose(1, 2).contiguous()
         if self._graph is None:
@@ -148,12 +155,26 @@ class DecodeSession:
         else:   # the position and the length are device buffers the graph advances
             c.append_at(layer, k_tok[0], v_tok[0], self._graph.slot)
             ctx = self._graph.ctx
-        q = query.reshape(1, h, d).to(torch.float16)
+        q = query.reshape(1, h, d)
+        if not (self._int4 and q.dtype == torch.bfloat16):      # (that kernel takes bf16 too)
+            q = q.to(torch.float16)
         out = torch.empty_like(q)
-        scales = dict(k_scales=c.k_scales[layer], v_scales=c.v_scales[layer]) if c.is_int8 else {}
+        scales = (dict(k_scales=c.k_scales[layer], v_scales=c.v_scales[layer])
+                  if c.is_int8 or self._int4 else {})
         registry.decode(self._kernel, out, q, c.k_cache[layer], c.v_cache[layer], c.block_table,
                         ctx, scaling, c.block_size, check=False, **scales)
         return out.view(1, 1, h, d).to(query.dtype)
+
+    def _attend_chunk(self, layer, query, key, value, scaling):
+        """A prompt chunk behind a cached prefix (4-bit cache): the chunk attends to the prefix's
+        cached values and causally to its own rows, which then join the cache."""
+        c = self.cache
+        pk, pv = c.gather(layer, torch.bfloat16 if key.dtype == torch.bfloat16 else torch.float16)
+        k = torch.cat([pk.permute(1, 0, 2)[None].to(key.dtype), key], dim=2)
+        v = torch.cat([pv.permute(1, 0, 2)[None].to(value.dtype), value], dim=2)
+        c.append_chunk(layer, key[0].permute(1, 0, 2).contiguous(),
+                       value[0].permute(1, 0, 2).contiguous())
+        return _causal_fp32(query, k, v, scaling).transpose(1, 2).contiguous()
 
 
 class DecodeGraph:
