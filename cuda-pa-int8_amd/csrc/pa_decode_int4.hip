@@ -7,32 +7,47 @@
 // scales and minima enter in fp32, at the scores and at the weights:
 //   scores   S[token][head]  = C'[tokens][32 dims] x Q^T[dims][16 heads]
 //   output   O^T[dim][head] += C^T[dims][32 tokens] x P^T[tokens][heads],  P = p s
-// A code c sits in the low bits of an fp16 element, where it is the subnormal number
-// c 2^-24, or 16 c 2^-24 from the upper half byte: masking is all the unpacking there is (5
-// instructions for 8 codes of K, 6 of V), and the matrix core takes subnormal
-// elements exactly.  The powers of two are put right in fp32, those of K in q (normalised
-// per head to at most 2^15 so that none of its bits are lost).
+// A code c sits in the low bits of an fp16 element, where it is a subnormal number: for K
+// c 2^-24, or 16 c 2^-24 from the upper half byte, and masks are all the unpacking there is (5
+// instructions for 8 codes); for V, whose bytes are put in token order first, 4 c 2^-24 or
+// 64 c 2^-24 (a shift and a mask each for the even and the odd dims).  The matrix core takes
+// subnormal elements exactly.  The powers of two are put right in fp32: those of K in q
+// (normalised per head to at most 2^15 so that none of its bits are lost), those of V when a
+// piece is finished.
 //
 // Lanes.  Lane l = (i = l & 15, g = l >> 4).  A tile is 64 tokens.  For K, lane (i, g) loads
 // quad i (tokens 4i .. 4i+3) of 8 dims 8 (4 step + g) ..: matrix row i of instruction n is token
 // 4i + n, and the scores of head h = i and tokens 16g + 4r + n come out in lane (h, g),
 // register r.  For V, lane (i, g) loads tokens 16g .. 16g + 15 of the dims 8i .. 8i + 7:
 // the weights that lane (h, g) holds are the operand as they are, no lane exchanges anything
-// but the running maximum, and output row i of instruction n is dim 8i + n.
+// but the running maximum, and output row i of instruction n is dim 8i + n.  A token's scale and
+// minimum are in one lane of its row, from where the score and weight instructions read them.
 //
 // Weights.  The reference point of the exponentials is the running maximum of score +
-// log2(s), less kShift: the P = p s stay at or below 2^kShift whatever the rows' scales.  P
-// enters as two fp16 numbers (its rounding and what that left), 22 bits together: with one
-// the outputs' error would grow threefold, as the codes are not centred.  sum p and sum p m are
-// fp32 sums of the unrounded weights.
+// log2(s), less kShift: the P = p s stay at or below 2^(kShift + kSlack) whatever the rows'
+// scales.  P enters as two fp16 numbers (its rounding and what that left), 22 bits together: with
+// one the outputs' error would grow threefold, as the codes are not centred.  sum p and sum p m
+// are fp32 sums of the unrounded weights.
 //
 // Work.  The tiles of all units (sequence, kv head, chunk of 16 HT query heads) form one list,
-// in that order, and the N waves of the launch take the ranges [i W / N, (i + 1) W / N) of its W
-// tiles: as even as tiles are, whatever the lengths, and found by every wave from
-// context_lens alone.  A unit inside one wave's range needs no merge at all; the pieces of a
-// unit that several waves share are merged through LDS, and those of a unit that several
-// work-groups share through memory, by the last of them to arrive (in two levels above
-// kMergeMax pieces).  All orders are fixed: the same bits every time.
+// in that order.  It is divided evenly among the work-groups, one a CU, and a work-group's part
+// among its waves: as even as tiles are, whatever the lengths, and found by every wave from
+// context_lens alone.  (Where lengths differ and the list is long, by cost rather than by tiles;
+// where units are few and short, a work-group takes one unit: both below.)  A unit inside one
+// wave's range needs no merge at all; the pieces of a unit that several waves share are merged
+// through LDS, and those of a unit that several work-groups share through memory, by the last of
+// them to arrive (in two levels above kMergeMax pieces).  All orders are fixed: the same bits
+// every time.
+//
+// What bounds it.  Long lists, the reads: the next tile's rows are loaded as this one's
+// registers fall free, eight waves a CU keep 64 to 128 KB under way, and the loop reads 6.3 to
+// 6.7 TB/s (large reads reach 7.0); V is read without being kept in the caches, and the wave that
+// is behind goes first on its SIMD.  A launch has about 2.5 us before its first rows arrive
+// (lengths, block ids, rows: three loads that wait for each other) and 5 to 9 us from the last
+// rows to the end where units are shared between work-groups, which is what bounds short ones.
+// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 7.1; 32 x 4096, 12/2 of 128: 14.8 (35.9 MB);
+// 8 x 32768, 32/8 of 128: 55 (5.2 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
+// 32/8 of 128: 66 (5.0 TB/s); 24 x 900-9000, 8/4 of 256: 37.4 (4.1 TB/s).
 #include <math.h>
 
 #include "pa_decode_kernels.hpp"
@@ -43,17 +58,12 @@ namespace pa {
 constexpr int kI4Waves = 8;          // waves of a work-group
 constexpr int kI4Groups = kInt4Groups;   // work-groups of a launch, at most: one a CU
 constexpr int kI4Tile = 64;          // tokens
-constexpr int kI4MinTiles = 1;       // tiles of a wave before another work-group is used
 constexpr int kMergeMax = 16;        // pieces merged at once
-constexpr float kShift = 14.f;
-constexpr float kSlack = 1.5f;
+// Tiles from which units of more than 16 heads take two head tiles (decode_int4_kernel).
+constexpr uint32_t kI4TwoTiles = 6u * kI4Groups * kI4Waves;
+constexpr float kShift = 14.f;       // the weights' upper end: 2^14 of fp16's 2^16, and
+constexpr float kSlack = 1.5f;       // how far a score may pass the reference before that moves
 constexpr float kCode24 = 16777216.f;   // 2^24: a code's element times this is the code
-
-// What a launch knows beside its pointers.
-struct I4Args {
-  int nchunk;
-  Int4DecodeShape sh;
-};
 
 // A tile of the list: tile t of the n of a unit (sequence, kv head, chunk of query heads).
 struct I4Tile {
@@ -111,8 +121,9 @@ __device__ __forceinline__ void dev_store4(__amdgpu_buffer_rsrc_t r, int off, f4
 
 // Eight tokens' scores: lanes E0 .. E0 + 7 of a row hold their scale and minimum, which the
 // instructions read from there (a row broadcast each).  z = m qn + s c.  The compiler does not
-// see what is inside: the first half (E0 = 0) waits out the matrix instructions behind c and
-// the two states before a broadcast of values just written, the second comes after it.
+// see what is inside: both halves wait the two states that a broadcast of values just written
+// needs, and the first (E0 = 0) waits out the matrix instructions behind c; the second comes
+// after it.
 template <int E0>
 __device__ __forceinline__ void score8(float (&z)[16], float m, float s, float qn, const f4_t* c) {
 #define PA_MUL(K, E) "v_mul_f32_dpp %" #K ", %8, %10 row_newbcast:" #E " row_mask:0xf bank_mask:0xf\n\t"
@@ -127,7 +138,7 @@ __device__ __forceinline__ void score8(float (&z)[16], float m, float s, float q
         PA_FMAC(3, 14, 3) PA_FMAC(4, 15, 4) PA_FMAC(5, 16, 5) PA_FMAC(6, 17, 6) PA_FMAC(7, 18, 7)
         : PA_OUT(0) : PA_IN(0));
   else
-    asm(PA_MUL(0, 8) PA_MUL(1, 9) PA_MUL(2, 10) PA_MUL(3, 11) PA_MUL(4, 12)
+    asm("s_nop 1\n\t" PA_MUL(0, 8) PA_MUL(1, 9) PA_MUL(2, 10) PA_MUL(3, 11) PA_MUL(4, 12)
         PA_MUL(5, 13) PA_MUL(6, 14) PA_MUL(7, 15) PA_FMAC(0, 11, 8) PA_FMAC(1, 12, 9)
         PA_FMAC(2, 13, 10) PA_FMAC(3, 14, 11) PA_FMAC(4, 15, 12) PA_FMAC(5, 16, 13)
         PA_FMAC(6, 17, 14) PA_FMAC(7, 18, 15)
@@ -173,60 +184,77 @@ __device__ __forceinline__ int select4(int a0, int a1, int a2, int a3, int k) {
   return (k & 2) ? hi : lo;
 }
 
+// What a wave knows of the lengths.  Lane l has the tiles of sequences l per .. l per + per - 1.
+struct I4Lens {
+  int per, lane_ctx;        // sequences a lane; the context of the lane's last
+  uint32_t incl, total;     // tiles of one (kv head, chunk): the lanes' running sum, and all
+  uint32_t longest;         // tiles of a sequence: the longest of this lane's
+  bool ragged;              // whether sequences differ
+};
+__device__ __forceinline__ I4Lens i4_lens(const int32_t* __restrict__ ctxl, int S, int cap) {
+  I4Lens r;
+  r.per = (S + kWave - 1) / kWave;
+  uint32_t mine = 0, shortest = ~0u;
+  r.longest = 0;
+  r.lane_ctx = 0;
+  for (int j = 0; j < r.per; ++j) {
+    const int s = (threadIdx.x & (kWave - 1)) * r.per + j;
+    r.lane_ctx = i4_clamp_ctx(ctxl[min(s, S - 1)], cap);
+    const uint32_t n = i4_tiles(r.lane_ctx);
+    mine += s < S ? n : 0u;
+    shortest = min(shortest, n);
+    r.longest = max(r.longest, n);
+  }
+  r.incl = wave_scan_dpp(mine);
+  r.total = (uint32_t)__builtin_amdgcn_readlane((int)r.incl, kWave - 1);
+  const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)shortest);
+  r.ragged = __any(shortest != first || r.longest != first);
+  return r;
+}
+
 template <int STEPS, int HT, bool BF>
-__global__ void __launch_bounds__(kI4Waves* kWave) __attribute__((amdgpu_waves_per_eu(2)))
-decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ ctxl, I4Args a,
-                   const uint16_t* __restrict__ q, const uint8_t* __restrict__ kc,
-                   const uint8_t* __restrict__ vc, const uint32_t* __restrict__ ks,
-                   const uint32_t* __restrict__ vs, uint16_t* __restrict__ out,
-                   float* __restrict__ ws, uint32_t* __restrict__ cnt) {
+__device__ __forceinline__ void decode_int4_body(
+    I4Smem<STEPS, HT>& sm, const I4Lens& lens, const int32_t* __restrict__ bt,
+    const int32_t* __restrict__ ctxl, const Int4DecodeShape& sh, const uint16_t* __restrict__ q,
+    const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+    const uint32_t* __restrict__ ks, const uint32_t* __restrict__ vs, uint16_t* __restrict__ out,
+    float* __restrict__ ws, uint32_t* __restrict__ cnt) {
   using G = I4Geo<STEPS, HT>;
   constexpr int T = G::T;
   // The waves' pieces of one unit are folded by all of them where a piece is one float4 a thread
   // (32 x 4096 at 12/2 heads 15.7 -> 14.9 us; with two, slower than by their first wave: 64
-  // ragged sequences at 32/1 24.6 against 26.4).
+  // sequences of median 2048 at 32/1 26.4 against 24.6).
   constexpr bool kTogether = T * HT == 1;
-  // the next unit's query is loaded a tile ahead where there are registers for it
+  // the next unit's query is loaded a tile ahead where there are registers for it (with more, the
+  // loop spills)
   constexpr bool kQueryAhead = STEPS * HT <= 4;
-  __shared__ I4Smem<STEPS, HT> sm;
   volatile int* prog = sm.progress;
-  const Int4DecodeShape& sh = a.sh;
+  const int nchunk = (sh.group + 16 * HT - 1) / (16 * HT);
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int S = sh.num_seqs, U = sh.num_kv_heads * a.nchunk, C = sh.head_dim / 8, D = sh.head_dim;
+  const int S = sh.num_seqs, U = sh.num_kv_heads * nchunk, C = sh.head_dim / 8, D = sh.head_dim;
   const int bs = 1 << sh.bs_log2;
   const int cap = sh.max_blocks << sh.bs_log2;
   const uint32_t cell_bytes = (uint32_t)(C * 4) << sh.bs_log2;   // bytes of a (block, head)
 
-  // ---- the wave's range.  Lane l sums the tiles of sequences l per .. l per + per - 1 (all
-  // counts fit 31 bits: the host has checked the table's capacity).
-  const int per = (S + kWave - 1) / kWave;
-  uint32_t mine = 0, shortest = ~0u, longest = 0;
-  int lane_ctx = 0;
-  for (int j = 0; j < per; ++j) {
-    const int s = lane * per + j;
-    lane_ctx = i4_clamp_ctx(ctxl[min(s, S - 1)], cap);
-    const uint32_t n = i4_tiles(lane_ctx);
-    mine += s < S ? n : 0u;
-    shortest = min(shortest, n);
-    longest = max(longest, n);
-  }
-  const uint32_t incl = wave_scan_dpp(mine);
-  const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1) * (uint32_t)U;
+  const int per = lens.per, lane_ctx = lens.lane_ctx;
+  const uint32_t incl = lens.incl;
+  const uint32_t tiles = lens.total * (uint32_t)U;
   // The list is divided by cost: 2 for a tile and 1 for a unit's start and end, where the units
-  // differ and a wave has tiles enough to make up for it; else evenly by tiles, as equal
-  // units divide best.
-  const uint32_t first_n = (uint32_t)__builtin_amdgcn_readfirstlane((int)shortest);
-  const bool ragged = __any(shortest != first_n || longest != first_n);
-  const bool weigh = ragged && tiles >= 4u * kI4Groups * kI4Waves;
+  // differ and a wave has tiles enough to make up for it (192 sequences of median 1024 and at most
+  // 8192 tokens 71.7 -> 65 us, 512 of 20 to 200 29.4 -> 28.6); else evenly by tiles, as equal units
+  // divide best (32 x 4096 by cost 16.3 -> 19.0).
+  const bool weigh = lens.ragged && tiles >= 4u * kI4Groups * kI4Waves;
   const uint32_t tile_cost = weigh ? 2u : 1u, unit_cost = weigh ? 1u : 0u;
   const uint32_t W = tiles * tile_cost + (uint32_t)(S * U) * unit_cost;
-  const uint32_t want = (tiles + kI4Waves * kI4MinTiles - 1) / (kI4Waves * kI4MinTiles);
+  // (another work-group as soon as every wave has a tile: with two each, 2000 tokens at 28/4 heads
+  // 10.7 -> 13.0 us)
+  const uint32_t want = (tiles + kI4Waves - 1) / kI4Waves;
   // Few short units get a work-group each: nothing then is merged through memory, which costs
   // about two tiles' time (4 x 100-512 tokens at 8/8 heads 10.4 -> 7.4 us).
   const uint32_t units = (uint32_t)(S * U);
   const uint32_t most = (tiles / (kI4Groups * kI4Waves) + 2) * kI4Waves;
-  const bool whole = units <= (uint32_t)kI4Groups && !__any(longest > most);
+  const bool whole = units <= (uint32_t)kI4Groups && !__any(lens.longest > most);
   const uint32_t groups = whole ? units : (want < kI4Groups ? want : kI4Groups);
   const uint32_t b = blockIdx.x;
   if (b >= groups) return;
@@ -272,8 +300,8 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
     t.ctx = ctx;
     t.n = n;
     t.t = c < unit_cost ? 0 : (int)((c - unit_cost) / tile_cost);
-    t.kvh = (int)(u / (uint32_t)a.nchunk);
-    t.ch = (int)u - t.kvh * a.nchunk;
+    t.kvh = (int)(u / (uint32_t)nchunk);
+    t.ch = (int)u - t.kvh * nchunk;
     return base * U + u * n + (uint32_t)t.t;
   };
   I4Tile cur, after;
@@ -282,8 +310,8 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
   if (whole) {
     const int seq = (int)(b / (uint32_t)U), u = (int)b - seq * U;
     cur.seq = seq;
-    cur.kvh = u / a.nchunk;
-    cur.ch = u - cur.kvh * a.nchunk;
+    cur.kvh = u / nchunk;
+    cur.ch = u - cur.kvh * nchunk;
     cur.ctx = i4_clamp_ctx(ctxl[seq], cap);
     cur.n = i4_tiles(cur.ctx);
     cur.ctx_next = 0;
@@ -297,7 +325,7 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
   auto advance = [&](I4Tile& t) {
     if (++t.t < t.n) return;
     t.t = 0;
-    if (++t.ch < a.nchunk) return;
+    if (++t.ch < nchunk) return;
     t.ch = 0;
     if (++t.kvh < sh.num_kv_heads) return;
     t.kvh = 0;
@@ -986,13 +1014,44 @@ decode_int4_kernel(const int32_t* __restrict__ bt, const int32_t* __restrict__ c
   }
 }
 
+// MAX_HT = 2 is for groups of more than 16 heads.  Two head tiles read and unpack such a unit's
+// rows once for both, but start, fold and merge twice the state, and one wave works where two
+// would.  Long lists take them (64 x 16384 tokens at 128/4 heads 145 us against 181, 64 x 8192
+// at 64/2 46.4 against 49.3), short ones do not (64 sequences of median 2048 at 32/1 21.8
+// against 24.8, 16 of 100-700 10.1 against 16.2); they meet near four to eight tiles a wave.  Wider rows
+// have no registers for a second set of outputs.
+//
+// The first arguments reach the waves in registers; the lengths are loaded while the rest come.
+template <int STEPS, int MAX_HT, bool BF>
+__global__ void __launch_bounds__(kI4Waves* kWave) __attribute__((amdgpu_waves_per_eu(2)))
+decode_int4_kernel(const int32_t* __restrict__ ctxl, int num_seqs, int max_blocks, int bs_log2,
+                   int num_kv_heads, int group, int head_dim, int num_blocks, float scale_log2,
+                   const int32_t* __restrict__ bt, const uint16_t* __restrict__ q,
+                   const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                   const uint32_t* __restrict__ ks, const uint32_t* __restrict__ vs,
+                   uint16_t* __restrict__ out, float* __restrict__ ws, uint32_t* __restrict__ cnt) {
+  const Int4DecodeShape sh{num_seqs, num_kv_heads * group, num_kv_heads, group, head_dim, num_blocks,
+                           max_blocks, bs_log2, scale_log2};
+  __shared__ I4Smem<STEPS, MAX_HT> sm;
+  const I4Lens lens = i4_lens(ctxl, sh.num_seqs, sh.max_blocks << sh.bs_log2);
+  if constexpr (MAX_HT > 1) {
+    if (lens.total * (uint32_t)sh.num_kv_heads >= kI4TwoTiles) {
+      decode_int4_body<STEPS, 2, BF>(sm, lens, bt, ctxl, sh, q, kc, vc, ks, vs, out, ws, cnt);
+      return;
+    }
+  }
+  decode_int4_body<STEPS, 1, BF>(reinterpret_cast<I4Smem<STEPS, 1>&>(sm), lens, bt, ctxl, sh, q, kc,
+                                 vc, ks, vs, out, ws, cnt);
+}
+
 namespace {
 
-template <int HT, bool BF>
+template <int MAX_HT, bool BF>
 hipError_t launch_tiles(const Int4Decode& l) {
-  const I4Args a{(l.shape.group + 16 * HT - 1) / (16 * HT), l.shape};
-  decode_int4_kernel<PA_INT4_STEPS, HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
-      l.block_table, l.context_lens, a, static_cast<const uint16_t*>(l.q),
+  decode_int4_kernel<PA_INT4_STEPS, MAX_HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
+      l.context_lens, l.shape.num_seqs, l.shape.max_blocks, l.shape.bs_log2, l.shape.num_kv_heads,
+      l.shape.group, l.shape.head_dim, l.shape.num_blocks, l.shape.scale_log2, l.block_table,
+      static_cast<const uint16_t*>(l.q),
       static_cast<const uint8_t*>(l.k_cache), static_cast<const uint8_t*>(l.v_cache),
       static_cast<const uint32_t*>(l.k_scales), static_cast<const uint32_t*>(l.v_scales),
       static_cast<uint16_t*>(l.out), l.workspace, l.counters);
@@ -1001,8 +1060,6 @@ hipError_t launch_tiles(const Int4Decode& l) {
 
 }  // namespace
 
-// Two head tiles where one unit then holds heads that would read its rows twice (their
-// second set of outputs needs the registers that wider heads use).
 template <>
 hipError_t launch_int4_decode_steps<PA_INT4_STEPS>(const Int4Decode& l) {
 #if PA_INT4_STEPS <= 4

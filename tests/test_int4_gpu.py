@@ -359,6 +359,31 @@ def test_decode_query_elements_decades_apart():
     close(out, *decode64(q, *cache, bt, [200, 31], 0.3), torch.float16)
 
 
+@pytest.mark.parametrize("heads,hkv,d,bs", [(32, 1, 64, 128), (40, 1, 128, 64), (71, 1, 96, 128),
+                                            (34, 2, 24, 32)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[300000, 1, 70001, 262144, 90000, 0, 64, 100000], [131072] * 6,
+                                  [131072] * 5 + [131008]])
+def test_decode_long_lists_of_wide_groups(heads, hkv, d, bs, dtype, lens):
+    """Groups of more than 16 heads with tiles for every wave to have six (12288 and one fewer
+    among the last two); sequences share the blocks of a small pool."""
+    import pa_int8
+
+    pool = 37
+    cache, _ = paged([pool * bs], hkv, d, bs, dtype, heads)
+    g = torch.Generator(device=DEV).manual_seed(heads + d)
+    bt = torch.randint(0, pool, (len(lens), -(-max(lens) // bs)), device=DEV, generator=g).int()
+    used = torch.isfinite(cache[2]).all(-1).all(-1).all(-1).nonzero()[:, 0].int()
+    assert used.numel() == pool
+    bt = used[bt.long()].contiguous()
+    q = torch.randn(len(lens), heads, d, device=DEV, generator=g).to(dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 9.0)
+    pa_int8.decode("int4", out, q, cache[0], cache[1], bt, ctx, d ** -0.5, bs, k_scales=cache[2],
+                   v_scales=cache[3], check=False)
+    close(out, *decode64(q, *cache, bt, lens, d ** -0.5), dtype)
+
+
 def test_decode_invalid_blocks_hold_no_tokens():
     import pa_int8
 
