@@ -14,8 +14,8 @@
 // the work-group that arrives last, when all others have read them, writes both.
 //
 // What bounds it is latency: the launch, two dependent loads, the scan and the stores.
-// MI355X, replayed from a graph: one token for each of 256 sequences 3.1 us (6.1 with 1024
-// threads, the searches and 64-bit shuffles of a first version), 64 prompts of 98,575 tokens 3.9
+// MI355X, replayed from a graph: one token for each of 256 sequences 3.3 us (6.1 with 1024
+// threads, the searches and 64-bit shuffles of a first version), 64 prompts of 98,575 tokens 3.8
 // (7.3), in place 6.8.
 #include "pa_decode_kernels.hpp"
 
@@ -27,12 +27,12 @@ constexpr int kFew = 4;
 
 struct ExtendArgs {
   int32_t* bt;
-  const int32_t *ctx, *nw, *free, *num_free;
+  const int32_t* free;
   int32_t *ctx_out, *num_free_out;
   int64_t *slots, *pos;
   int32_t *cu, *status;
   uint32_t* counter;
-  int seqs, max_blocks, bs_log2, rows, free_cap;
+  int rows;
   bool in_place;
 };
 
@@ -53,24 +53,33 @@ __device__ __forceinline__ long long wave_scan64(uint32_t v) {
   return ((long long)wave_scan_dpp(v >> 16) << 16) + wave_scan_dpp(v & 0xFFFFu);
 }
 
+// (The first arguments reach the waves in registers; the lengths are loaded while the rest come.)
 template <int PER>
-__global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
+__global__ void __launch_bounds__(kExtThreads)
+extend_kernel(const int32_t* ctx_in, const int32_t* new_in, const int32_t* num_free, int seqs,
+              int max_blocks, int bs_log2, int free_cap, ExtendArgs a) {
   constexpr int NW = kExtThreads / kWave;
   extern __shared__ int lds[];               // cu, first, ctx of each sequence
   __shared__ long long wsum[2][NW];
   __shared__ int wflag[NW];
   __shared__ bool last;
-  const int S = a.seqs, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid >> 6;
-  const int s0 = tid * PER, bs = 1 << a.bs_log2;
-  const int nfree = *a.num_free;
+  const int S = seqs, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid >> 6;
+  const int s0 = tid * PER, bs = 1 << bs_log2;
+  int z = 0;
+  asm volatile("" : "+v"(z));      // (loaded as the lengths are, with them)
+  const int nfree_lane = num_free[z];
   int c[PER], n[PER], need[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int s = min(s0 + i, S - 1);
-    c[i] = a.ctx[s];
-    n[i] = a.nw[s];
+    c[i] = ctx_in[s];
+    n[i] = new_in[s];
   }
-  int bad = 0;
+  const int nfree = __builtin_amdgcn_readfirstlane(nfree_lane);
+  // (here by now; left alone, the compiler asks for them behind the barrier)
+  asm volatile("" : : "s"(a.bt), "s"(a.free), "s"(a.slots), "s"(a.pos), "s"(a.cu), "s"(a.status),
+               "s"(a.ctx_out), "s"(a.num_free_out), "s"(a.rows), "s"((int)a.in_place));
+  int bad = nfree < 0 || nfree > free_cap ? kExtendBadLength : 0;
   bool many = false;
   long long xn = 0, xb = 0;   // inclusive sums up to this thread, within the wave
 #pragma unroll
@@ -80,9 +89,9 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
       if (s0 + i < S) bad |= kExtendBadLength;
       n[i] = 0;
     } else {
-      const long long have = ((long long)c[i] + bs - 1) >> a.bs_log2;
-      const long long want = ((long long)c[i] + n[i] + bs - 1) >> a.bs_log2;
-      if (want > a.max_blocks || (long long)c[i] + n[i] > INT32_MAX) bad |= kExtendRowFull;
+      const long long have = ((long long)c[i] + bs - 1) >> bs_log2;
+      const long long want = ((long long)c[i] + n[i] + bs - 1) >> bs_log2;
+      if (want > max_blocks || (long long)c[i] + n[i] > INT32_MAX) bad |= kExtendRowFull;
       need[i] = (int)(want - have);
       many |= n[i] > kFew;
     }
@@ -93,6 +102,7 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
     wsum[0][wv] = xn;
     wsum[1][wv] = xb;
   }
+  // (all reads of what may be updated in place are over at the barrier)
   // one bit for each reason, and one for a long row of new tokens
   const int f1 = __any(bad & kExtendBadLength) ? kExtendBadLength : 0;
   const int f2 = __any(bad & kExtendRowFull) ? kExtendRowFull : 0;
@@ -117,8 +127,7 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
     arrived = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const bool search = (st & 16) != 0;
   st &= 15;
-  if (nfree < 0 || nfree > a.free_cap) st |= kExtendBadLength;
-  else if (allb > nfree) st |= kExtendNoBlocks;
+  if (nfree >= 0 && nfree <= free_cap && allb > nfree) st |= kExtendNoBlocks;
   if (alln > a.rows) st |= kExtendNoRows;
   const int live = st ? 0 : (int)alln, blocks = st ? 0 : (int)allb;
 #pragma unroll
@@ -133,12 +142,12 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
     if (blockIdx.x == 0 && s0 + i < S) {
       if (a.cu) a.cu[s0 + i] = st ? 0 : (int)xn;
       if (!search && !st) {
-        const int have = (c[i] + bs - 1) >> a.bs_log2;
-        int32_t* row = a.bt + (size_t)(s0 + i) * a.max_blocks;
+        const int have = (c[i] + bs - 1) >> bs_log2;
+        int32_t* row = a.bt + (size_t)(s0 + i) * max_blocks;
         for (int k = 0; k < n[i]; ++k) {
-          const int p = c[i] + k, b = (p >> a.bs_log2) - have;
-          const int blk = b < 0 ? row[p >> a.bs_log2] : a.free[nfree - 1 - ((int)xb + b)];
-          if (b >= 0 && (p & (bs - 1)) == 0) row[p >> a.bs_log2] = blk;
+          const int p = c[i] + k, b = (p >> bs_log2) - have;
+          const int blk = b < 0 ? row[p >> bs_log2] : a.free[nfree - 1 - ((int)xb + b)];
+          if (b >= 0 && (p & (bs - 1)) == 0) row[p >> bs_log2] = blk;
           a.slots[(int)xn + k] = (int64_t)blk * bs + (p & (bs - 1));
           if (a.pos) a.pos[(int)xn + k] = p;
         }
@@ -157,8 +166,8 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
     for (; r < live; r += stride) {
       const int s = last_at_most(cu, S, r);
       const int c0 = ctx[s], p = c0 + (r - cu[s]);
-      const int b = (p >> a.bs_log2) - ((c0 + bs - 1) >> a.bs_log2);
-      int32_t* entry = a.bt + (size_t)s * a.max_blocks + (p >> a.bs_log2);
+      const int b = (p >> bs_log2) - ((c0 + bs - 1) >> bs_log2);
+      int32_t* entry = a.bt + (size_t)s * max_blocks + (p >> bs_log2);
       const int blk = b < 0 ? *entry : a.free[nfree - 1 - (first[s] + b)];
       if (b >= 0 && (p & (bs - 1)) == 0) *entry = blk;    // (a new block's first token)
       a.slots[r] = (int64_t)blk * bs + (p & (bs - 1));
@@ -188,13 +197,9 @@ __global__ void __launch_bounds__(kExtThreads) extend_kernel(ExtendArgs a) {
 }
 
 hipError_t launch_extend(const ExtendLaunch& l) {
-  auto overlap = [&](const int32_t* x, const int32_t* y, int n) { return x < y + n && y < x + n; };
-  const bool in_place = overlap(l.context_lens_out, l.context_lens, l.num_seqs) ||
-                        overlap(l.num_free_out, l.num_free, 1);
-  ExtendArgs a{l.block_table, l.context_lens, l.new_lens, l.free_blocks, l.num_free,
-               l.context_lens_out, l.num_free_out, l.slot_mapping, l.positions, l.cu_seqlens,
-               l.status, l.counter, l.num_seqs, l.max_blocks,
-               __builtin_ctz((unsigned)l.block_size), l.num_rows, l.free_capacity, in_place};
+  const bool in_place = l.context_lens_out == l.context_lens || l.num_free_out == l.num_free;
+  ExtendArgs a{l.block_table, l.free_blocks, l.context_lens_out, l.num_free_out, l.slot_mapping,
+               l.positions, l.cu_seqlens, l.status, l.counter, l.num_rows, in_place};
   // One row a thread; in place fewer work-groups, as their arrivals are counted in one word,
   // one after another (98,575 rows: 64 work-groups 8.3 us, 256 6.8).
   const int most = in_place ? 256 : 512;
@@ -203,7 +208,9 @@ hipError_t launch_extend(const ExtendLaunch& l) {
   const size_t lds = 3 * sizeof(int) * l.num_seqs;
   const int per = (l.num_seqs + kExtThreads - 1) / kExtThreads;
   auto* k = per <= 1 ? extend_kernel<1> : (per <= 4 ? extend_kernel<4> : extend_kernel<kExtPer>);
-  k<<<grid, kExtThreads, lds, l.stream>>>(a);
+  k<<<grid, kExtThreads, lds, l.stream>>>(l.context_lens, l.new_lens, l.num_free, l.num_seqs,
+                                         l.max_blocks, __builtin_ctz((unsigned)l.block_size),
+                                         l.free_capacity, a);
   return hipGetLastError();
 }
 

@@ -87,6 +87,21 @@ size_t workspace_bytes_of(const pa::Int4DecodeShape& s) {
   }
 }
 
+// Whether any of the first `outs` ranges meets another range.
+struct Range {
+  const void* p;
+  size_t bytes;
+};
+template <int N>
+bool outputs_overlap(const Range (&r)[N], int outs) {
+  for (int i = 0; i < outs; ++i)
+    for (int j = i + 1; j < N; ++j) {
+      const auto a = reinterpret_cast<uintptr_t>(r[i].p), b = reinterpret_cast<uintptr_t>(r[j].p);
+      if (r[i].bytes && r[j].bytes && a < b + r[j].bytes && b < a + r[i].bytes) return true;
+    }
+  return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -175,6 +190,17 @@ pa_status_t pa_extend_block_tables(int32_t* block_table, const int32_t* context_
     return PA_ERR_NULL_POINTER;
   if (!counters || counter_bytes < sizeof(uint32_t) || !aligned(counters, 4))
     return PA_ERR_WORKSPACE;
+  // Work-groups read the inputs while others write the outputs: only the lengths and the free
+  // count may be updated in place.
+  const size_t lens = 4 * (size_t)num_seqs, rows = 8 * (size_t)num_rows;
+  const Range ranges[] = {
+      {block_table, lens * (size_t)max_blocks_per_seq}, {slot_mapping, rows},
+      {positions, positions ? rows : 0}, {cu_seqlens, cu_seqlens ? lens + 4 : 0}, {status, 4},
+      {context_lens_out, lens}, {num_free_out, 4},
+      {context_lens, context_lens == context_lens_out ? 0 : lens},
+      {num_free, num_free == num_free_out ? 0 : (size_t)4}, {new_lens, lens},
+      {free_blocks, 4 * (size_t)free_capacity}};
+  if (outputs_overlap(ranges, 7)) return PA_ERR_BAD_SHAPE;
   pa::ExtendLaunch l{block_table, context_lens, new_lens, free_blocks, num_free, context_lens_out,
                      num_free_out, slot_mapping, positions, cu_seqlens, status,
                      static_cast<uint32_t*>(counters), num_seqs, max_blocks_per_seq, block_size,

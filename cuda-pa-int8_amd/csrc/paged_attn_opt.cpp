@@ -555,7 +555,7 @@ void extend_block_tables(at::Tensor block_table, at::Tensor context_lens, at::Te
   hipStream_t stream =
       at::hip::getCurrentHIPStreamMasqueradingAsCUDA(block_table.get_device()).stream();
   at::Tensor cnt = counters_for(block_table, stream, kMinCounterBytes);
-  check_status(pa_extend_block_tables(
+  const pa_status_t st = pa_extend_block_tables(
       block_table.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
       new_lens.data_ptr<int32_t>(), free_blocks.data_ptr<int32_t>(), num_free.data_ptr<int32_t>(),
       ctx_out.data_ptr<int32_t>(), free_out.data_ptr<int32_t>(), slot_mapping.data_ptr<int64_t>(),
@@ -563,7 +563,9 @@ void extend_block_tables(at::Tensor block_table, at::Tensor context_lens, at::Te
       cu_seqlens.has_value() ? cu_seqlens->data_ptr<int32_t>() : nullptr,
       status.data_ptr<int32_t>(), (int32_t)S, (int32_t)block_table.size(1), (int32_t)block_size,
       (int32_t)slot_mapping.size(0), (int32_t)free_blocks.size(0), cnt.data_ptr(), cnt.numel(),
-      reinterpret_cast<pa_stream_t>(stream)));
+      reinterpret_cast<pa_stream_t>(stream));
+  TORCH_CHECK(st != PA_ERR_BAD_SHAPE, "an output overlaps another tensor, or a size is out of range");
+  check_status(st);
 }
 
 // Checks shared by the cache-write ops; `int8` selects the cache dtypes and

@@ -373,7 +373,7 @@ pa_status_t pa_paged_decode_attn_int4(
  *     token get slot -1, which the cache writes skip, and position 0;
  *   - cu_seqlens [num_seqs + 1] receives the first row of each sequence and their number,
  *     context_lens_out the new lengths, *num_free_out what is left (either may be the input:
- *     updated in place).
+ *     updated in place; no output may overlap anything else).
  * *status receives 0, or the sum of the reasons below; then nothing was placed: block_table,
  * the lengths and the free count keep their values, and every row has slot -1.
  * positions and cu_seqlens may be NULL.  block_size is a power of two up to 128,

@@ -169,6 +169,38 @@ def test_optional_outputs_and_several_steps():
     check(t, want)
 
 
+def test_several_calls_captured_into_a_graph():
+    """Two steps and a chunk, in place, replayed: each replay goes on from the last one."""
+    ctx, bs = [5, 0, 47, 16], 16
+    t = tensors(ctx, [80] * 4, bs, 9, 0, 700, 11)
+    steps = [[1, 1, 1, 1], [0, 12, 1, 0], [2, 1, 0, 2]]
+    news = [torch.tensor(n, dtype=torch.int32, device=DEV) for n in steps]
+    outs = [{k: torch.empty_like(t[k]) for k in ("slots", "pos", "cu", "st")} for _ in steps]
+    calls = [{**t, **o, "new": n} for o, n in zip(outs, news)]
+    start = {k: t[k].clone() for k in ("bt", "ctx", "nfree")}
+    for c in calls:                        # (outside a capture first)
+        run(c, bs)
+    torch.cuda.synchronize()
+    for k, v in start.items():
+        t[k].copy_(v)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for c in calls:
+            run(c, bs)
+    for _ in range(3):
+        state = [t["bt"].tolist(), t["ctx"].tolist(), int(t["nfree"])]
+        g.replay()
+        torch.cuda.synchronize()
+        for c, n in zip(calls, steps):
+            want = plain(state[0], state[1], n, t["free"].tolist(), state[2], 700, bs)
+            state = [want[0], want[1], want[2]]
+            assert want[6] == 0 and c["st"].item() == 0
+            assert c["slots"].tolist() == want[3] and c["pos"].tolist() == want[4]
+            assert c["cu"].tolist() == want[5]
+        assert t["bt"].tolist() == state[0] and t["ctx"].tolist() == state[1]
+        assert t["nfree"].item() == state[2]
+
+
 def test_refusals():
     import pa_int8
 
@@ -186,6 +218,10 @@ def test_refusals():
                       (dict(bt=t["bt"].cpu()), "CUDA")]:
         with pytest.raises(RuntimeError, match=match):
             call(**kw)
+    with pytest.raises(RuntimeError, match="overlaps"):   # (an output is no other input)
+        pa_int8.extend_block_tables(*[t[n] for n in args], 16, context_lens_out=t["new"])
+    with pytest.raises(RuntimeError, match="overlaps"):
+        call(st=t["nfree"])
     n = 4097
     z = torch.zeros(n, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError, match="at most 4096"):

@@ -90,6 +90,24 @@ def test_extend_refusals(lib, kw, status):
     assert lib.pa_extend_block_tables(*extend_args(**kw)) == status
 
 
+APART = {n: P + 4096 * (i + 1) for i, n in enumerate(
+    ("bt", "ctx", "new", "free", "nfree", "ctxo", "nfo", "slots", "pos", "cu", "st"))}
+
+
+@pytest.mark.parametrize("out", ["bt", "ctxo", "nfo", "slots", "pos", "cu", "st"])
+def test_extend_outputs_stand_alone(lib, out):
+    """An output that shares memory with another tensor is refused, by one element too."""
+    size = dict(bt=48, ctx=12, new=12, free=36, nfree=4, ctxo=12, nfo=4, slots=64, pos=64, cu=16,
+                st=4)
+    for other, n in size.items():
+        if other == out:
+            continue
+        for at in (APART[other] + n - 4, APART[other] - size[out] + 4):
+            if at == APART[other] and (out, other) in (("ctxo", "ctx"), ("nfo", "nfree")):
+                continue                   # (updated in place)
+            assert lib.pa_extend_block_tables(*extend_args(**{**APART, out: at})) == SHAPE, other
+
+
 def test_ops_reject_cpu_tensors(built):
     import pa_int8
 
