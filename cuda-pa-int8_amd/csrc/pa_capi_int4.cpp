@@ -87,6 +87,31 @@ size_t workspace_bytes_of(const pa::Int4DecodeShape& s) {
   }
 }
 
+pa_status_t decode_int4(
+    void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+    const void* v_scales, const int32_t* block_table, const int32_t* context_lens, float scale,
+    int32_t block_size, int32_t num_seqs, int32_t num_heads, int32_t head_dim,
+    int32_t num_kv_heads, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t bf16,
+    void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
+    uint64_t* report, uint32_t tag, pa_stream_t stream) {
+  pa::Int4DecodeShape s;
+  const pa_status_t st = decode_shape(num_seqs, num_heads, head_dim, num_kv_heads, num_blocks,
+                                      block_size, max_blocks_per_seq, scale, &s);
+  if (st != PA_OK || num_seqs == 0) return st;
+  if (!out || !q || !k_cache || !v_cache || !k_scales || !v_scales || !context_lens ||
+      (!block_table && max_blocks_per_seq > 0))
+    return PA_ERR_NULL_POINTER;
+  for (const void* p : {static_cast<const void*>(out), q, k_cache, v_cache, k_scales, v_scales})
+    if (!aligned(p, 16)) return PA_ERR_BAD_SHAPE;
+  if (!counters || counter_bytes < pa_decode_int4_counter_bytes() || !aligned(counters, 256) ||
+      !workspace || workspace_bytes < workspace_bytes_of(s) || !aligned(workspace, 256))
+    return PA_ERR_WORKSPACE;
+  pa::Int4Decode l{out, q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens,
+                   bf16 != 0, static_cast<uint32_t*>(counters), static_cast<float*>(workspace), report, tag, s,
+                   reinterpret_cast<hipStream_t>(stream)};
+  return launch_decode(l) == hipSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
 // Whether any of the first `outs` ranges meets another range.
 struct Range {
   const void* p;
@@ -153,22 +178,25 @@ pa_status_t pa_paged_decode_attn_int4(
     int32_t num_kv_heads, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t bf16,
     void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
     pa_stream_t stream) {
-  pa::Int4DecodeShape s;
-  const pa_status_t st = decode_shape(num_seqs, num_heads, head_dim, num_kv_heads, num_blocks,
-                                      block_size, max_blocks_per_seq, scale, &s);
-  if (st != PA_OK || num_seqs == 0) return st;
-  if (!out || !q || !k_cache || !v_cache || !k_scales || !v_scales || !context_lens ||
-      (!block_table && max_blocks_per_seq > 0))
-    return PA_ERR_NULL_POINTER;
-  for (const void* p : {static_cast<const void*>(out), q, k_cache, v_cache, k_scales, v_scales})
-    if (!aligned(p, 16)) return PA_ERR_BAD_SHAPE;
-  if (!counters || counter_bytes < pa_decode_int4_counter_bytes() || !aligned(counters, 256) ||
-      !workspace || workspace_bytes < workspace_bytes_of(s) || !aligned(workspace, 256))
-    return PA_ERR_WORKSPACE;
-  pa::Int4Decode l{out, q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens,
-                   bf16 != 0, static_cast<uint32_t*>(counters), static_cast<float*>(workspace), s,
-                   reinterpret_cast<hipStream_t>(stream)};
-  return launch_decode(l) == hipSuccess ? PA_OK : PA_ERR_LAUNCH;
+  return decode_int4(out, q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens, scale,
+                     block_size, num_seqs, num_heads, head_dim, num_kv_heads, num_blocks,
+                     max_blocks_per_seq, bf16, counters, counter_bytes, workspace,
+                     workspace_bytes, nullptr, 0, stream);
+}
+
+pa_status_t pa_paged_decode_attn_int4_checked(
+    void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+    const void* v_scales, const int32_t* block_table, const int32_t* context_lens, float scale,
+    int32_t block_size, int32_t num_seqs, int32_t num_heads, int32_t head_dim,
+    int32_t num_kv_heads, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t bf16,
+    void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
+    uint64_t* report, uint32_t tag, pa_stream_t stream) {
+  if (!report) return PA_ERR_NULL_POINTER;
+  if (!aligned(report, 8)) return PA_ERR_BAD_SHAPE;
+  return decode_int4(out, q, k_cache, v_cache, k_scales, v_scales, block_table, context_lens, scale,
+                     block_size, num_seqs, num_heads, head_dim, num_kv_heads, num_blocks,
+                     max_blocks_per_seq, bf16, counters, counter_bytes, workspace,
+                     workspace_bytes, report, tag, stream);
 }
 
 pa_status_t pa_extend_block_tables(int32_t* block_table, const int32_t* context_lens,

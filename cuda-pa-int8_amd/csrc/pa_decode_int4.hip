@@ -45,9 +45,9 @@
 // is behind goes first on its SIMD.  A launch has about 2.5 us before its first rows arrive
 // (lengths, block ids, rows: three loads that wait for each other) and 5 to 9 us from the last
 // rows to the end where units are shared between work-groups, which is what bounds short ones.
-// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 7.1; 32 x 4096, 12/2 of 128: 14.8 (35.9 MB);
+// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 7.1; 32 x 4096, 12/2 of 128: 14.4 (36 MB);
 // 8 x 32768, 32/8 of 128: 55 (5.2 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
-// 32/8 of 128: 66 (5.0 TB/s); 24 x 900-9000, 8/4 of 256: 37.4 (4.1 TB/s).
+// 32/8 of 128: 66 (5.0 TB/s); 24 x 900-9000, 8/4 of 256: 37.2 (4.2 TB/s).
 #include <math.h>
 
 #include "pa_decode_kernels.hpp"
@@ -99,6 +99,7 @@ struct alignas(16) I4Smem {
   } piece[2];
   int last2;
 };
+constexpr int kI4Check = 256;        // beside the block size's log2: a checked call
 constexpr int kHasTiles = 1, kHead = 2, kHeadEnds = 4, kTail = 8;
 
 __device__ __forceinline__ int i4_clamp_ctx(int c, int cap) { return c < 0 ? 0 : (c > cap ? cap : c); }
@@ -184,22 +185,33 @@ __device__ __forceinline__ int select4(int a0, int a1, int a2, int a3, int k) {
   return (k & 2) ? hi : lo;
 }
 
+// Lengths and block table, which nothing in the launch writes: uniform reads stay scalar loads,
+// whatever stores come before them.
+typedef const __attribute__((address_space(4))) int32_t* const_i32;
+__device__ __forceinline__ const_i32 as_const(const int32_t* p) {
+  return (const_i32)reinterpret_cast<uintptr_t>(p);
+}
+
 // What a wave knows of the lengths.  Lane l has the tiles of sequences l per .. l per + per - 1.
 struct I4Lens {
   int per, lane_ctx;        // sequences a lane; the context of the lane's last
   uint32_t incl, total;     // tiles of one (kv head, chunk): the lanes' running sum, and all
   uint32_t longest;         // tiles of a sequence: the longest of this lane's
   bool ragged;              // whether sequences differ
+  bool empty;               // whether one holds no token
 };
-__device__ __forceinline__ I4Lens i4_lens(const int32_t* __restrict__ ctxl, int S, int cap) {
+__device__ __forceinline__ I4Lens i4_lens(const_i32 ctxl, int S, int cap) {
   I4Lens r;
   r.per = (S + kWave - 1) / kWave;
   uint32_t mine = 0, shortest = ~0u;
   r.longest = 0;
   r.lane_ctx = 0;
+  int least = 1;
   for (int j = 0; j < r.per; ++j) {
     const int s = (threadIdx.x & (kWave - 1)) * r.per + j;
-    r.lane_ctx = i4_clamp_ctx(ctxl[min(s, S - 1)], cap);
+    const int ctx = ctxl[min(s, S - 1)];
+    least = min(least, ctx);
+    r.lane_ctx = i4_clamp_ctx(ctx, cap);
     const uint32_t n = i4_tiles(r.lane_ctx);
     mine += s < S ? n : 0u;
     shortest = min(shortest, n);
@@ -209,13 +221,14 @@ __device__ __forceinline__ I4Lens i4_lens(const int32_t* __restrict__ ctxl, int 
   r.total = (uint32_t)__builtin_amdgcn_readlane((int)r.incl, kWave - 1);
   const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)shortest);
   r.ragged = __any(shortest != first || r.longest != first);
+  r.empty = __any(least < 1);
   return r;
 }
 
 template <int STEPS, int HT, bool BF>
 __device__ __forceinline__ void decode_int4_body(
-    I4Smem<STEPS, HT>& sm, const I4Lens& lens, const int32_t* __restrict__ bt,
-    const int32_t* __restrict__ ctxl, const Int4DecodeShape& sh, const uint16_t* __restrict__ q,
+    I4Smem<STEPS, HT>& sm, const I4Lens& lens, const_i32 bt, const_i32 ctxl,
+    const Int4DecodeShape& sh, const uint16_t* __restrict__ q,
     const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const uint32_t* __restrict__ ks, const uint32_t* __restrict__ vs, uint16_t* __restrict__ out,
     float* __restrict__ ws, uint32_t* __restrict__ cnt) {
@@ -228,7 +241,6 @@ __device__ __forceinline__ void decode_int4_body(
   // the next unit's query is loaded a tile ahead where there are registers for it (with more, the
   // loop spills)
   constexpr bool kQueryAhead = STEPS * HT <= 4;
-  volatile int* prog = sm.progress;
   const int nchunk = (sh.group + 16 * HT - 1) / (16 * HT);
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -343,7 +355,7 @@ __device__ __forceinline__ void decode_int4_body(
     Ids r{{-1, -1, -1, -1}};
     if (t.ctx > 0) {
       const int lastb = (t.ctx - 1) >> sh.bs_log2;
-      const int32_t* row = bt + (size_t)t.seq * sh.max_blocks;
+      const const_i32 row = bt + (size_t)t.seq * sh.max_blocks;
 #pragma unroll
       for (int j = 0; j < 4; ++j) r.b[j] = row[min((t.t * kI4Tile + 16 * j) >> sh.bs_log2, lastb)];
     }
@@ -410,7 +422,8 @@ __device__ __forceinline__ void decode_int4_body(
 
   // ---- the query of a unit: raw rows, then the matrix operand.  Scores in its units: those
   // of base 2 are cs z, cs >= 0 (a negative scale turns the query round).
-  uint4 qr[HT][STEPS], qa[HT][STEPS];
+  uint4 qr[HT][STEPS];
+  u4_t qa[HT][STEPS];
   float cs[HT], qn[HT];
   auto load_q = [&](const I4Tile& t) {
 #pragma unroll
@@ -420,7 +433,7 @@ __device__ __forceinline__ void decode_int4_body(
           q + ((size_t)t.seq * sh.num_heads + t.kvh * sh.group + hh) * D);
 #pragma unroll
       for (int j = 0; j < STEPS; ++j)
-        qa[ht][j] = *reinterpret_cast<const uint4*>(row + k_chunk(j));
+        qa[ht][j] = *reinterpret_cast<const u4_t*>(row + k_chunk(j));
     }
   };
   auto convert_q = [&]() {
@@ -430,7 +443,7 @@ __device__ __forceinline__ void decode_int4_body(
       float mx = 0.f, sum = 0.f;
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        if (4 * j + g >= C) qa[ht][j] = make_uint4(0, 0, 0, 0);
+        if (4 * j + g >= C) qa[ht][j] = (u4_t){0, 0, 0, 0};
         const uint32_t w[4] = {qa[ht][j].x, qa[ht][j].y, qa[ht][j].z, qa[ht][j].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -439,7 +452,7 @@ __device__ __forceinline__ void decode_int4_body(
           sum += lo + hi;
         }
         // (the second pass widens the rows again, as there are no registers to keep them wide)
-        asm volatile("" : "+v"(qa[ht][j].x), "+v"(qa[ht][j].y), "+v"(qa[ht][j].z), "+v"(qa[ht][j].w));
+        asm volatile("" : "+v"(qa[ht][j]));
       }
       mx = head_max(mx);
       sum = head_sum(sum);
@@ -632,6 +645,14 @@ __device__ __forceinline__ void decode_int4_body(
   };
 
   // ---- the wave's tiles
+  // (relaxed atomics of the work-group: a volatile's system scope waits for every load under way,
+  // the next tile's rows too; 8 x 1000 tokens at 32/8 heads 11.0 -> 10.4 us without that wait)
+  auto set_progress = [&](int k) {
+    __hip_atomic_store(&sm.progress[wv], k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  auto progress_of = [&](int w) {
+    return __hip_atomic_load(&sm.progress[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
   int state = count > 0 ? kHasTiles : 0;
   const int t0 = cur.t;
   if (count > 0) {
@@ -651,7 +672,7 @@ __device__ __forceinline__ void decode_int4_body(
       advance(nx);
       idn = load_ids(nx);
     }
-    prog[wv] = 0;
+    set_progress(0);
     reset();
     convert_q();
     if (kQueryAhead && count > 1 && nx.t == 0) load_q(nx);
@@ -681,10 +702,10 @@ __device__ __forceinline__ void decode_int4_body(
     // (head: the unit was begun before the wave, whose tiles it still holds without a break)
     for (int k = 0; k < count - 1; ++k) {
       // Of the SIMD's two waves the one behind goes first (left alone, the older does).
-      const int other = __builtin_amdgcn_readfirstlane(prog[wv ^ 4]);
+      const int other = __builtin_amdgcn_readfirstlane(progress_of(wv ^ 4));
       if (k <= other) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
-      prog[wv] = k + 1;
+      set_progress(k + 1);
       w = locate(nx, idn);
       I4Tile nn = nx;
       if (k + 2 < count) {
@@ -703,6 +724,11 @@ __device__ __forceinline__ void decode_int4_body(
       if (kQueryAhead && k + 2 < count && nx.t == 0) load_q(nx);
     }
     process(std::false_type(), live, nx, w);
+    // (a query asked for may still be on its way as far as the compiler knows: were its registers
+    // used for this tile, the tile would wait for it)
+    if constexpr (kQueryAhead)
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) asm volatile("" : : "v"(qa[0][j]));
     finish(cur.t == cur.n - 1, (state & kHead) && cur.t == t0 + count - 1);
     if (kTogether && (state & (kHead | kTail)) == kTail) {
       to_slot();
@@ -1021,19 +1047,30 @@ __device__ __forceinline__ void decode_int4_body(
 // against 24.8, 16 of 100-700 10.1 against 16.2); they meet near four to eight tiles a wave.  Wider rows
 // have no registers for a second set of outputs.
 //
-// The first arguments reach the waves in registers; the lengths are loaded while the rest come.
+// The first arguments reach the waves in registers; the lengths are loaded while the rest come, whether
+// the call is checked among the first.
 template <int STEPS, int MAX_HT, bool BF>
 __global__ void __launch_bounds__(kI4Waves* kWave) __attribute__((amdgpu_waves_per_eu(2)))
-decode_int4_kernel(const int32_t* __restrict__ ctxl, int num_seqs, int max_blocks, int bs_log2,
+decode_int4_kernel(const int32_t* __restrict__ lengths, int num_seqs, int max_blocks, int bs_check,
                    int num_kv_heads, int group, int head_dim, int num_blocks, float scale_log2,
-                   const int32_t* __restrict__ bt, const uint16_t* __restrict__ q,
+                   const int32_t* __restrict__ table, const uint16_t* __restrict__ q,
                    const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                    const uint32_t* __restrict__ ks, const uint32_t* __restrict__ vs,
-                   uint16_t* __restrict__ out, float* __restrict__ ws, uint32_t* __restrict__ cnt) {
+                   uint16_t* __restrict__ out, float* __restrict__ ws, uint32_t* __restrict__ cnt,
+                   uint64_t* __restrict__ report, uint32_t tag) {
+  const int bs_log2 = bs_check & 255;
   const Int4DecodeShape sh{num_seqs, num_kv_heads * group, num_kv_heads, group, head_dim, num_blocks,
                            max_blocks, bs_log2, scale_log2};
   __shared__ I4Smem<STEPS, MAX_HT> sm;
+  const const_i32 ctxl = as_const(lengths), bt = as_const(table);
   const I4Lens lens = i4_lens(ctxl, sh.num_seqs, sh.max_blocks << sh.bs_log2);
+  // A checked call's answer goes out at once, while the launch goes on; all leave where it is no.
+  if (bs_check & kI4Check) {
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+      __hip_atomic_store(report, ((uint64_t)tag << 32) | (lens.empty ? 0u : 1u), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_SYSTEM);
+    if (lens.empty) return;
+  }
   if constexpr (MAX_HT > 1) {
     if (lens.total * (uint32_t)sh.num_kv_heads >= kI4TwoTiles) {
       decode_int4_body<STEPS, 2, BF>(sm, lens, bt, ctxl, sh, q, kc, vc, ks, vs, out, ws, cnt);
@@ -1049,12 +1086,13 @@ namespace {
 template <int MAX_HT, bool BF>
 hipError_t launch_tiles(const Int4Decode& l) {
   decode_int4_kernel<PA_INT4_STEPS, MAX_HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
-      l.context_lens, l.shape.num_seqs, l.shape.max_blocks, l.shape.bs_log2, l.shape.num_kv_heads,
-      l.shape.group, l.shape.head_dim, l.shape.num_blocks, l.shape.scale_log2, l.block_table,
+      l.context_lens, l.shape.num_seqs, l.shape.max_blocks,
+      l.shape.bs_log2 | (l.report != nullptr ? kI4Check : 0), l.shape.num_kv_heads, l.shape.group,
+      l.shape.head_dim, l.shape.num_blocks, l.shape.scale_log2, l.block_table,
       static_cast<const uint16_t*>(l.q),
       static_cast<const uint8_t*>(l.k_cache), static_cast<const uint8_t*>(l.v_cache),
       static_cast<const uint32_t*>(l.k_scales), static_cast<const uint32_t*>(l.v_scales),
-      static_cast<uint16_t*>(l.out), l.workspace, l.counters);
+      static_cast<uint16_t*>(l.out), l.workspace, l.counters, l.report, l.tag);
   return hipGetLastError();
 }
 

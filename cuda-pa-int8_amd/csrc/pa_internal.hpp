@@ -249,6 +249,8 @@ struct Int4Decode {
   bool bf16;           // q and out
   uint32_t* counters;  // 3 * kInt4Groups, zero between launches
   float* workspace;    // 2 * kInt4Groups pieces
+  uint64_t* report;    // where the check of the lengths goes, or NULL for none
+  uint32_t tag;
   Int4DecodeShape shape;
   hipStream_t stream;
 };

@@ -109,12 +109,13 @@ LengthSlot& length_slot() {
   return *s;
 }
 
-// Smallest, largest and mean context length through a kernel that writes them where the
-// host polls.  False (nothing done) where that does not apply: lengths elsewhere
-// than on q's device or not dense (a later check reports them), a stream under
-// capture, no host memory.
-bool polled_range(const at::Tensor& ctx, const at::Tensor& q, int32_t* mn, int32_t* mx,
-                  int32_t* mean) {
+// A check of the context lengths through a kernel that writes `words` results where the
+// host polls: `launch` (slot memory, tag, stream) starts it, and results[i] is the low half of
+// word i.  False (nothing done) where that does not apply: lengths elsewhere than on q's device
+// or not dense (a later check reports them), a stream under capture, no host memory.
+template <class Launch>
+bool polled(const at::Tensor& ctx, const at::Tensor& q, int words, int32_t* results,
+            Launch launch) {
   if (!ctx.is_cuda() || ctx.get_device() != q.get_device() || !ctx.is_contiguous() ||
       ctx.numel() > INT32_MAX)
     return false;
@@ -127,16 +128,17 @@ bool polled_range(const at::Tensor& ctx, const at::Tensor& q, int32_t* mn, int32
   if (mem == nullptr) return false;
   volatile uint64_t* w = mem;
   const uint32_t tag = ++slot.tag;
-  w[0] = w[1] = w[2] = (uint64_t)(tag - 1) << 32;   // whatever the slot holds is not this call's tag
+  for (int i = 0; i < words; ++i)
+    w[i] = (uint64_t)(tag - 1) << 32;   // whatever the slot holds is not this call's tag
   std::atomic_thread_fence(std::memory_order_seq_cst);
-  check_status(pa_context_lens_range(ctx.data_ptr<int32_t>(), (int32_t)ctx.numel(), mem, tag,
-                                     reinterpret_cast<pa_stream_t>(stream)));
+  check_status(launch(mem, tag, stream));
   // The stream may have other work before the kernel: poll for about as long as
   // a blocked wait costs more than it saves, then wait on the stream.
   const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(1);
   auto done = [&] {
-    return (uint32_t)(w[0] >> 32) == tag && (uint32_t)(w[1] >> 32) == tag &&
-           (uint32_t)(w[2] >> 32) == tag;
+    bool all = true;
+    for (int i = 0; i < words; ++i) all = all && (uint32_t)(w[i] >> 32) == tag;
+    return all;
   };
   for (int spin = 0; !done(); ++spin) {
     __builtin_ia32_pause();
@@ -147,10 +149,23 @@ bool polled_range(const at::Tensor& ctx, const at::Tensor& q, int32_t* mn, int32
       TORCH_CHECK(done(), "context_lens check: the kernel's result did not arrive");
     }
   }
-  *mn = (int32_t)(uint32_t)w[0];
-  *mx = (int32_t)(uint32_t)w[1];
-  *mean = (int32_t)(uint32_t)w[2];
+  for (int i = 0; i < words; ++i) results[i] = (int32_t)(uint32_t)w[i];
   ++slot.polled;
+  return true;
+}
+
+// Smallest, largest and mean context length.
+bool polled_range(const at::Tensor& ctx, const at::Tensor& q, int32_t* mn, int32_t* mx,
+                  int32_t* mean) {
+  int32_t r[3];
+  if (!polled(ctx, q, 3, r, [&](uint64_t* mem, uint32_t tag, hipStream_t stream) {
+        return pa_context_lens_range(ctx.data_ptr<int32_t>(), (int32_t)ctx.numel(), mem, tag,
+                                     reinterpret_cast<pa_stream_t>(stream));
+      }))
+    return false;
+  *mn = r[0];
+  *mx = r[1];
+  *mean = r[2];
   return true;
 }
 
@@ -424,11 +439,6 @@ void paged_decode_attn_int4(at::Tensor out, at::Tensor q, at::Tensor k_cache, at
   }
   TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && block_table.size(1) <= INT32_MAX,
               "q or block_table too large");
-  if (check_context && context_lens.numel() > 0) {
-    int32_t mn = 0, mx = 0, mean = 0;
-    if (!polled_range(context_lens, q, &mn, &mx, &mean)) mn = context_lens.min().item<int32_t>();
-    TORCH_CHECK(mn >= 1, "context_lens must be >= 1 (empty sequences unsupported)");
-  }
   const int32_t S = (int32_t)q.size(0), H = (int32_t)q.size(1), D = (int32_t)q.size(2);
   const int32_t Hkv = (int32_t)k_cache.size(1), MB = (int32_t)block_table.size(1);
   const at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
@@ -436,12 +446,25 @@ void paged_decode_attn_int4(at::Tensor out, at::Tensor q, at::Tensor k_cache, at
   const size_t need = pa_decode_int4_workspace_bytes(S, H, D, Hkv, (int32_t)block_size, MB);
   at::Tensor cnt = counters_for(q, stream, pa_decode_int4_counter_bytes());
   at::Tensor ws = at::empty({(int64_t)std::max<size_t>(need, 256)}, q.options().dtype(at::kByte));
-  check_status(pa_paged_decode_attn_int4(
-      out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
-      v_scales.data_ptr(), block_table.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
-      (float)scale, (int32_t)block_size, S, H, D, Hkv, (int32_t)k_cache.size(0), MB,
-      q.scalar_type() == at::kBFloat16, cnt.data_ptr(), cnt.numel(), ws.data_ptr(), ws.numel(),
-      reinterpret_cast<pa_stream_t>(stream)));
+  auto run = [&](auto entry, auto... report) {
+    return entry(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr<int32_t>(),
+                 context_lens.data_ptr<int32_t>(), (float)scale, (int32_t)block_size, S, H, D, Hkv,
+                 (int32_t)k_cache.size(0), MB, (int32_t)(q.scalar_type() == at::kBFloat16),
+                 cnt.data_ptr(), (size_t)cnt.numel(), ws.data_ptr(), (size_t)ws.numel(), report...,
+                 reinterpret_cast<pa_stream_t>(stream));
+  };
+  if (check_context && S > 0) {
+    // The decode launch checks the lengths itself, and leaves `out` alone where they fail.
+    int32_t ok = 0;
+    const bool asked = polled(context_lens, q, 1, &ok, [&](uint64_t* mem, uint32_t tag, hipStream_t) {
+      return run(pa_paged_decode_attn_int4_checked, mem, tag);
+    });
+    if (!asked) ok = context_lens.min().item<int32_t>() >= 1;
+    TORCH_CHECK(ok, "context_lens must be >= 1 (empty sequences unsupported)");
+    if (asked) return;
+  }
+  check_status(run(pa_paged_decode_attn_int4));
 }
 
 void check_int4_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_cache,

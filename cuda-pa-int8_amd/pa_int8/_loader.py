@@ -123,6 +123,8 @@ PROTOTYPES = {
     "pa_decode_int4_workspace_bytes": (_sz, [_i32] * 6),
     "pa_paged_decode_attn_int4": (ctypes.c_int, [_p] * 8 + [_f32] + [_i32] * 8 +
                                   [_p, _sz, _p, _sz, _p]),
+    "pa_paged_decode_attn_int4_checked": (ctypes.c_int, [_p] * 8 + [_f32] + [_i32] * 8 +
+                                          [_p, _sz, _p, _sz, _p, ctypes.c_uint32, _p]),
     "pa_extend_block_tables": (ctypes.c_int, [_p] * 11 + [_i32] * 5 + [_p, _sz, _p]),
     "pa_reshape_and_cache_f16": (ctypes.c_int, [_p, _p, _i64, _i64, _i64, _i64, _p, _i32, _i32,
                                                 _i32, _p, _p, _i32, _i32, _i32, _p]),

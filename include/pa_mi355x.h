@@ -363,6 +363,18 @@ pa_status_t pa_paged_decode_attn_int4(
     void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
     pa_stream_t stream);
 
+/* The same with the check of the lengths in it: *report = tag << 32 | 1 where all are >= 1;
+ * else tag << 32, and out is left as it is.  The word is stored early in the launch, once, at
+ * system scope: with `report` in coherent host memory the caller polls it for its tag (as
+ * pa_context_lens_range; nothing is stored where num_seqs is 0). */
+pa_status_t pa_paged_decode_attn_int4_checked(
+    void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+    const void* v_scales, const int32_t* block_table, const int32_t* context_lens, float scale,
+    int32_t block_size, int32_t num_seqs, int32_t num_heads, int32_t head_dim,
+    int32_t num_kv_heads, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t bf16,
+    void* counters, size_t counter_bytes, void* workspace, size_t workspace_bytes,
+    uint64_t* report, uint32_t tag, pa_stream_t stream);
+
 /* Room for a batch's new tokens.  NEW API: what a serving loop does on the host between
  * steps, in one launch and without a read-back, for any cache type.  Sequence s holds
  * context_lens[s] tokens and gets new_lens[s] more (both >= 0):

@@ -457,6 +457,44 @@ def test_decode_checked_names_and_refusals():
             run(**kw)
 
 
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 300])
+def test_checked_decode_finds_an_empty_sequence(n):
+    """Wherever it is, with the output left alone; the call after it, and one whose lengths
+    come from work still queued, run as the unchecked call does."""
+    import pa_int8
+
+    cache, bt = paged([20 + i % 7 for i in range(n)], 2, 64, 16, torch.float16, n)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    q = torch.randn(n, 8, 64, device=DEV, generator=g).half()
+    ctx = torch.tensor([20 + i % 7 for i in range(n)], dtype=torch.int32, device=DEV)
+    want = pa_int8.decode("int4", torch.empty_like(q), q, cache[0], cache[1], bt, ctx, 0.1, 16,
+                          k_scales=cache[2], v_scales=cache[3], check=False)
+    checked = lambda out, c: pa_int8.VARIANTS_INT4["int4"](out, q, *cache, bt, c, 0.1, 16)  # noqa: E731
+    for bad in (0, -5, -2 ** 31):
+        for at in {0, n // 2, n - 1}:
+            c = ctx.clone()
+            c[at] = bad
+            out = torch.full_like(q, 7)
+            with pytest.raises(RuntimeError, match="context_lens must be >= 1"):
+                checked(out, c)
+            assert bool((out == 7).all())
+            assert torch.equal(checked(out, ctx), want)
+    a = torch.randn(4096, 4096, device=DEV)
+    for _ in range(60):
+        a = (a @ a) * 1e-3
+    late = (ctx.float() + 0 * a[0, 0].nan_to_num()).to(torch.int32)
+    assert torch.equal(checked(torch.empty_like(q), late), want)
+    pa_int8.ext()._length_slot(1)              # no memory to poll for the next check
+    assert torch.equal(checked(torch.empty_like(q), ctx), want)
+    pa_int8.ext()._length_slot(1)
+    out = torch.full_like(q, 7)
+    with pytest.raises(RuntimeError, match="context_lens must be >= 1"):
+        checked(out, c)
+    assert bool((out == 7).all())
+    none = pa_int8.VARIANTS_INT4["int4"](q[:0].clone(), q[:0], *cache, bt[:0], ctx[:0], 0.1, 16)
+    assert none.numel() == 0
+
+
 def test_decode_same_bits_again_and_on_another_stream():
     import pa_int8
 

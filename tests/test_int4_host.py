@@ -60,6 +60,15 @@ def test_decode_refusals(lib, kw, status):
     assert lib.pa_paged_decode_attn_int4(*decode_args(**kw)) == status
 
 
+@pytest.mark.parametrize("kw,report,status", [
+    (dict(), None, NULL), (dict(), P + 4, SHAPE), (dict(q=None), P, NULL), (dict(wb=0), P, WORKSPACE),
+    (dict(seqs=0), P, OK), (dict(d=12), P, UNSUPPORTED)])
+def test_checked_decode_refusals(lib, kw, report, status):
+    args = decode_args(**kw)
+    args[-1:-1] = [report, 7]
+    assert lib.pa_paged_decode_attn_int4_checked(*args) == status
+
+
 def test_decode_sizes(lib):
     ws = lib.pa_decode_int4_workspace_bytes
     assert lib.pa_decode_int4_counter_bytes() <= 256 << 10
