@@ -45,9 +45,9 @@
 // is behind goes first on its SIMD.  A launch has about 2.5 us before its first rows arrive
 // (lengths, block ids, rows: three loads that wait for each other) and 5 to 9 us from the last
 // rows to the end where units are shared between work-groups, which is what bounds short ones.
-// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 7.1; 32 x 4096, 12/2 of 128: 14.4 (36 MB);
+// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 6.7; 32 x 4096, 12/2 of 128: 14.0 (36 MB);
 // 8 x 32768, 32/8 of 128: 55 (5.2 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
-// 32/8 of 128: 66 (5.0 TB/s); 24 x 900-9000, 8/4 of 256: 37.2 (4.2 TB/s).
+// 32/8 of 128: 65 (5.1 TB/s); 24 x 900-9000, 8/4 of 256: 33.2 (4.7 TB/s).
 #include <math.h>
 
 #include "pa_decode_kernels.hpp"
@@ -70,11 +70,27 @@ struct I4Tile {
   int seq, kvh, ch, t, n, ctx, ctx_next;
 };
 
-// float4s a lane keeps of a piece: [head tile][16-chunk tile][row r][half].
-template <int STEPS, int HT>
+// Groups of at most 8 heads leave columns of the products free.
+// kPack, heads wider than 64: a finished piece holds the second half of each 8 dims in columns
+// 8 .. 15, so that pieces are half as large in LDS and memory.  kPack4, at most 4 such heads: the
+// four quads of columns hold a quarter each.
+// kPair, heads of at most 64 dims, which leave half of the rows of the output product free too:
+// matrix rows i and i + 8 are chunk i of a lane row's tokens 16g .. 16g + 7 and 16g + 8 .., columns
+// c and c + 8 head c's weights of the same, and the blocks where they meet count.  Half the
+// softmax, the conversions of V and the products of a tile; a finished piece holds the second half
+// of each 8 dims in lanes 32 ...
+// (kPair: 64 x 2000-16000 tokens at 32/8 heads of 64 86 -> 73 us, 16 x 500-8000 at 14/2 14.2 -> 12.6.
+// kPack and kPack4: 24 x 900-9000 at 8/4 heads of 256 37.1 -> 33.2, one of 131072 at 8/1 of 128
+// 16.6 -> 14.4, 32 x 4096 at 12/2 14.4 -> 14.0.)
+constexpr int kWhole = 0, kPack = 1, kPair = 2, kPack4 = 3;
+// Items of a head tile and 16 chunks.
+constexpr int mode_items(int mode) { return mode == kWhole ? 8 : (mode == kPack4 ? 2 : 4); }
+
+// A piece: items of 64 lanes x 4 dims, [head tile][16-chunk tile][item], kWhole's [row r][half].
+template <int STEPS, int HT, int MODE>
 struct I4Geo {
   static constexpr int T = (STEPS + 3) / 4;
-  static constexpr int NF = 8 * T * HT;
+  static constexpr int NF = mode_items(MODE) * T * HT;
   static constexpr int kPieceFloats = NF * kWave * 4;
   static constexpr int kMlFloats = 2 * 16 * HT;
   static constexpr size_t kSlotFloats = kPieceFloats + kMlFloats;
@@ -86,9 +102,9 @@ struct I4Unit {
   int n, seq, kvh, ch;
 };
 
-template <int STEPS, int HT>
+template <int STEPS, int HT, int MODE>
 struct alignas(16) I4Smem {
-  using G = I4Geo<STEPS, HT>;
+  using G = I4Geo<STEPS, HT, MODE>;
   f4_t acc[kI4Waves][G::NF][kWave];
   f2_t ml[kI4Waves][16 * HT];
   I4Unit head[kI4Waves], tail[kI4Waves];
@@ -180,6 +196,32 @@ __device__ __forceinline__ float row_max(float v) {
   v = fmaxf(v, dpp_mov<kRowHalfMirror>(v));
   return fmaxf(v, dpp_mov<kRowMirror>(v));
 }
+constexpr int kRowRor4 = 0x124, kRowRor8 = 0x128, kRowRor12 = 0x12C, kQuadReverse = 0x1B;
+// Of a head's two columns.
+__device__ __forceinline__ float pair_max8(float v) { return fmaxf(v, dpp_mov<kRowRor8>(v)); }
+__device__ __forceinline__ float pair_sum8(float v) { return v + dpp_mov<kRowRor8>(v); }
+// v, in columns 8 .. 15 u's of columns 0 .. 7.
+template <int CTRL = kRowRor8, int BANKS = 0xC>
+__device__ __forceinline__ float upper_from(float v, float u) {
+  return bitsf((uint32_t)__builtin_amdgcn_update_dpp((int)fbits(v), (int)fbits(u), CTRL, 0xF, BANKS,
+                                                     false));
+}
+// a, b, c and d of columns 0 .. 3 in the four quads of columns.
+__device__ __forceinline__ float quads_from(float a, float b, float c, float d) {
+  return upper_from<kRowRor12, 0x8>(
+      upper_from<kRowRor8, 0x4>(upper_from<kRowRor4, 0x2>(a, b), c), d);
+}
+// v, in the quads of BANKS that of the lane 4 further or back in its 8.
+template <int BANKS>
+__device__ __forceinline__ uint32_t other_quad(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)dpp_mov_u<kRowHalfMirror>(v),
+                                               kQuadReverse, 0xF, BANKS, false);
+}
+// The value that lane N of the quad holds.
+template <int N>
+__device__ __forceinline__ float quad_bcast(float v) {
+  return dpp_mov<N * 0x55>(v);
+}
 __device__ __forceinline__ int select4(int a0, int a1, int a2, int a3, int k) {
   const int lo = (k & 1) ? a1 : a0, hi = (k & 1) ? a3 : a2;
   return (k & 2) ? hi : lo;
@@ -225,19 +267,20 @@ __device__ __forceinline__ I4Lens i4_lens(const_i32 ctxl, int S, int cap) {
   return r;
 }
 
-template <int STEPS, int HT, bool BF>
+template <int STEPS, int HT, int MODE, bool BF>
 __device__ __forceinline__ void decode_int4_body(
-    I4Smem<STEPS, HT>& sm, const I4Lens& lens, const_i32 bt, const_i32 ctxl,
+    I4Smem<STEPS, HT, MODE>& sm, const I4Lens& lens, const_i32 bt, const_i32 ctxl,
     const Int4DecodeShape& sh, const uint16_t* __restrict__ q,
     const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const uint32_t* __restrict__ ks, const uint32_t* __restrict__ vs, uint16_t* __restrict__ out,
     float* __restrict__ ws, uint32_t* __restrict__ cnt) {
-  using G = I4Geo<STEPS, HT>;
-  constexpr int T = G::T;
-  // The waves' pieces of one unit are folded by all of them where a piece is one float4 a thread
-  // (32 x 4096 at 12/2 heads 15.7 -> 14.9 us; with two, slower than by their first wave: 64
+  using G = I4Geo<STEPS, HT, MODE>;
+  constexpr bool PAIR = MODE == kPair, PACK = MODE == kPack, PACK4 = MODE == kPack4;
+  constexpr int T = G::T, I = mode_items(MODE);
+  // The waves' pieces of one unit are folded by all of them where a piece is at most one float4 a
+  // thread (32 x 4096 at 12/2 heads 15.7 -> 14.9 us; with two, slower than by their first wave: 64
   // sequences of median 2048 at 32/1 26.4 against 24.6).
-  constexpr bool kTogether = T * HT == 1;
+  constexpr bool kTogether = G::NF <= kI4Waves;
   // the next unit's query is loaded a tile ahead where there are registers for it (with more, the
   // loop spills)
   constexpr bool kQueryAhead = STEPS * HT <= 4;
@@ -377,7 +420,8 @@ __device__ __forceinline__ void decode_int4_body(
     return Where{select4(sb[0], sb[1], sb[2], sb[3], i16 >> 2),
                  select4(sb[0], sb[1], sb[2], sb[3], g), select4(lv[0], lv[1], lv[2], lv[3], g)};
   };
-  uint4 kr[STEPS], vr[T][4];
+  constexpr int VQ = PAIR ? 2 : 4;         // quads of V's tokens a lane loads
+  uint4 kr[STEPS], vr[T][VQ];
   uint32_t ksr, vsr;
   // Byte offset of step j's 8 dims of K (of a query) for this lane.  Opaque to the compiler,
   // which would otherwise keep each sum of such offsets in registers through the loop.
@@ -404,16 +448,16 @@ __device__ __forceinline__ void decode_int4_body(
     vsr = vs[at];
   };
   auto load_v = [&](const I4Tile& t, const Where& w) {
-    const int off = (t.t * kI4Tile + 16 * g) & (bs - 1);
+    const int off = (t.t * kI4Tile + 16 * g + (PAIR ? i16 & 8 : 0)) & (bs - 1);
     const uint8_t* p = vc + (uint64_t)(uint32_t)(w.v * sh.num_kv_heads + t.kvh) * cell_bytes +
                        (uint32_t)quad_offset(off, C);
 #pragma unroll
     for (int tt = 0; tt < T; ++tt) {
-      uint32_t c = min(16 * tt + i16, C - 1) * 16;
+      uint32_t c = min(16 * tt + (PAIR ? i16 & 7 : i16), C - 1) * 16;
       asm volatile("" : "+v"(c));
       const uint8_t* row = p + c;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < VQ; ++k) {
         vr[tt][k] = load_stream<uint4>(row);
         row += v_step;
       }
@@ -428,7 +472,7 @@ __device__ __forceinline__ void decode_int4_body(
   auto load_q = [&](const I4Tile& t) {
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      const int hh = min(t.ch * 16 * HT + ht * 16 + i16, sh.group - 1);
+      const int hh = min(t.ch * 16 * HT + ht * 16 + (PAIR ? i16 & 7 : i16), sh.group - 1);
       const uint8_t* row = reinterpret_cast<const uint8_t*>(
           q + ((size_t)t.seq * sh.num_heads + t.kvh * sh.group + hh) * D);
 #pragma unroll
@@ -515,27 +559,46 @@ __device__ __forceinline__ void decode_int4_body(
     const uint32_t kp = mine_live ? ksr : 0u, vp = mine_live ? vsr : 0u;
     const float s_k = widen_lo<false>(kp), m_k = widen_hi<false>(kp);
     const float s_v = widen_lo<false>(vp), m_v = widen_hi<false>(vp);
+    // (PAIR: the pairs of the lane's 8 tokens, four in each quad of its 8 lanes)
+    const uint32_t kpj[2] = {other_quad<0xA>(kp), other_quad<0x5>(kp)};
+    const uint32_t vpj[2] = {other_quad<0xA>(vp), other_quad<0x5>(vp)};
     if constexpr (kMore) load_scales(nx, wn);
     // (2^-24: fp16's smallest step, for rows of one value, whose scale is 0)
     const float log_s = __builtin_amdgcn_logf(fmaxf(row_max(s_v), 0x1p-24f));
     const bool full = __all(live >= 16);
-    h8_t phi[HT][2], plo[HT][2];
+    h8_t phi[HT][VQ / 2], plo[HT][VQ / 2];
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      float z[16];
-      score8<0>(z, m_k, s_k, qn[ht], sc[ht]);
-      score8<8>(z, m_k, s_k, qn[ht], sc[ht]);
+      constexpr int E = PAIR ? 8 : 16;       // the lane's tokens
+      float z[E];
+      if constexpr (PAIR) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) x[n] = (i16 & 8) ? sc[ht][n][2 + j] : sc[ht][n][j];
+          const float mj = widen_hi<false>(kpj[j]), sj = widen_lo<false>(kpj[j]);
+          z[4 * j + 0] = __builtin_fmaf(quad_bcast<0>(sj), x[0], quad_bcast<0>(mj) * qn[ht]);
+          z[4 * j + 1] = __builtin_fmaf(quad_bcast<1>(sj), x[1], quad_bcast<1>(mj) * qn[ht]);
+          z[4 * j + 2] = __builtin_fmaf(quad_bcast<2>(sj), x[2], quad_bcast<2>(mj) * qn[ht]);
+          z[4 * j + 3] = __builtin_fmaf(quad_bcast<3>(sj), x[3], quad_bcast<3>(mj) * qn[ht]);
+        }
+      } else {
+        score8<0>(z, m_k, s_k, qn[ht], sc[ht]);
+        score8<8>(z, m_k, s_k, qn[ht], sc[ht]);
+      }
       if (!full) {
         asm volatile("");   // (a branch: most tiles are full)
+        const int mine = PAIR ? live - (i16 & 8) : live;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = e < live ? z[e] : kNegInf;
+        for (int e = 0; e < E; ++e) z[e] = e < mine ? z[e] : kNegInf;
       }
       float mx = fmaxf(z[0], z[1]);
 #pragma unroll
-      for (int e = 2; e < 16; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
+      for (int e = 2; e < E; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
       // (a tile without tokens: -inf, also where cs is 0)
       mx = mx == kNegInf ? kNegInf : __builtin_fmaf(mx, cs[ht], log_s);
-      mx = head_max(mx);
+      mx = head_max(PAIR ? pair_max8(mx) : mx);
       // The reference moves when it is passed by kSlack: the weights then stay below 2^16.
       const bool move = mx > M[ht] + kSlack;
       if (__any(move)) {
@@ -550,15 +613,31 @@ __device__ __forceinline__ void decode_int4_body(
       }
       const float ref = M[ht] == kNegInf ? 0.f : M[ht] - kShift;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
+      for (int hf = 0; hf < E / 8; ++hf) {
         float p[8], w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = exp2f_fast(__builtin_fmaf(z[8 * hf + e], cs[ht], -ref));
           L[ht] += p[e];
         }
-        if (hf == 0) weight8<0>(w, B[ht], m_v, s_v, p);
-        else weight8<8>(w, B[ht], m_v, s_v, p);
+        if constexpr (PAIR) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float mj = widen_hi<false>(vpj[j]), sj = widen_lo<false>(vpj[j]);
+            w[4 * j + 0] = quad_bcast<0>(sj) * p[4 * j + 0];
+            w[4 * j + 1] = quad_bcast<1>(sj) * p[4 * j + 1];
+            w[4 * j + 2] = quad_bcast<2>(sj) * p[4 * j + 2];
+            w[4 * j + 3] = quad_bcast<3>(sj) * p[4 * j + 3];
+            B[ht] = __builtin_fmaf(quad_bcast<0>(mj), p[4 * j + 0], B[ht]);
+            B[ht] = __builtin_fmaf(quad_bcast<1>(mj), p[4 * j + 1], B[ht]);
+            B[ht] = __builtin_fmaf(quad_bcast<2>(mj), p[4 * j + 2], B[ht]);
+            B[ht] = __builtin_fmaf(quad_bcast<3>(mj), p[4 * j + 3], B[ht]);
+          }
+        } else if (hf == 0) {
+          weight8<0>(w, B[ht], m_v, s_v, p);
+        } else {
+          weight8<8>(w, B[ht], m_v, s_v, p);
+        }
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           // (towards zero: the second number holds what that leaves)
@@ -575,7 +654,7 @@ __device__ __forceinline__ void decode_int4_body(
 #pragma unroll
     for (int tt = 0; tt < T; ++tt) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
+      for (int hf = 0; hf < VQ / 2; ++hf) {
         const uint4 a0 = vr[tt][2 * hf], a1 = vr[tt][2 * hf + 1];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -604,27 +683,75 @@ __device__ __forceinline__ void decode_int4_body(
   auto to_piece = [&]() {
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      L[ht] = head_sum(L[ht]);
-      B[ht] = head_sum(B[ht]);
+      L[ht] = head_sum(PAIR ? pair_sum8(L[ht]) : L[ht]);
+      B[ht] = head_sum(PAIR ? pair_sum8(B[ht]) : B[ht]);
+      if constexpr (PACK) {
+        M[ht] = upper_from(M[ht], M[ht]);
+        L[ht] = upper_from(L[ht], L[ht]);
+        B[ht] = upper_from(B[ht], B[ht]);
+      }
+      if constexpr (PACK4) {
+        M[ht] = quads_from(M[ht], M[ht], M[ht], M[ht]);
+        L[ht] = quads_from(L[ht], L[ht], L[ht], L[ht]);
+        B[ht] = quads_from(B[ht], B[ht], B[ht], B[ht]);
+      }
 #pragma unroll
       for (int tt = 0; tt < T; ++tt)
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < (MODE == kWhole ? 8 : 4); ++n)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < (PACK4 ? 2 : 4); ++r) {
+            float v = acc[ht][tt][n][r];
+            if constexpr (PAIR) {
+              // both token halves' sums, dim n in lanes 0 - 31 and dim n + 4 in the others
+              const auto w = __builtin_amdgcn_permlane32_swap(fbits(v), fbits(acc[ht][tt][n + 4][r]),
+                                                              false, false);
+              v = bitsf((uint32_t)w[0]) + dpp_mov<kRowRor8>(bitsf((uint32_t)w[1]));
+            }
+            if constexpr (PACK) v = upper_from(v, acc[ht][tt][n + 4][r]);
+            if constexpr (PACK4)
+              v = quads_from(v, acc[ht][tt][n + 4][r], acc[ht][tt][n][r + 2], acc[ht][tt][n + 4][r + 2]);
             acc[ht][tt][n][r] =
-                __builtin_fmaf(acc[ht][tt][n][r], (n & 1) ? kCode24 / 64.f : kCode24 / 4.f, B[ht]);
+                __builtin_fmaf(v, (n & 1) ? kCode24 / 64.f : kCode24 / 4.f, B[ht]);
+          }
     }
   };
   auto piece4 = [&](int ht, int tt, int r, int half) {
     return (f4_t){acc[ht][tt][4 * half][r], acc[ht][tt][4 * half + 1][r],
                   acc[ht][tt][4 * half + 2][r], acc[ht][tt][4 * half + 3][r]};
   };
+  // Item f of a piece: four dims of the column's head.
+  auto item4 = [&](int ht, int tt, int f) {
+    return MODE != kWhole ? piece4(ht, tt, f, 0) : piece4(ht, tt, f >> 1, f & 1);
+  };
+  // Its head tile, and which 8 dims and which half of them it is.
+  auto item_head = [&](int f) { return f / (I * T); };
+  auto item_chunk = [&](int f) {
+    if constexpr (PAIR) return 4 * (g & 1) + f;
+    const int row = PACK4 ? (f & 1) + 2 * (i16 >> 3) : (PACK ? f & 3 : (f & 7) >> 1);
+    return ((f / I) % T) * 16 + 4 * g + row;
+  };
+  auto item_half = [&](int f) {
+    return PAIR ? g >> 1 : (PACK ? i16 >> 3 : (PACK4 ? (i16 >> 2) & 1 : f & 1));
+  };
+  const int column = PACK ? i16 & 7 : (PACK4 ? i16 & 3 : i16);   // the column's head
   auto write_out = [&](int seq, int kvh, int ch) {
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
-      const int hh = ch * 16 * HT + ht * 16 + i16;
+      const int hh = ch * 16 * HT + ht * 16 + column;
       const float inv = L[ht] != 0.f ? 1.f / L[ht] : 0.f;
+      if constexpr (MODE != kWhole) {
+#pragma unroll
+        for (int f = 0; f < G::NF; ++f) {
+          const int chunk = item_chunk(f);
+          if (hh >= sh.group || chunk >= C) continue;
+          const f4_t v = item4(ht, f / I, f % I);
+          *reinterpret_cast<uint2*>(out + ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D +
+                                    chunk * 8 + 4 * item_half(f)) =
+              make_uint2(pack2<BF>(v[0] * inv, v[1] * inv), pack2<BF>(v[2] * inv, v[3] * inv));
+        }
+        continue;
+      }
       int gq = g;
       asm volatile("" : "+v"(gq));   // (as k_chunk)
 #pragma unroll
@@ -682,8 +809,8 @@ __device__ __forceinline__ void decode_int4_body(
 #pragma unroll
         for (int tt = 0; tt < T; ++tt)
 #pragma unroll
-          for (int f = 0; f < 8; ++f)
-            sm.acc[wv][(ht * T + tt) * 8 + f][lane] = piece4(ht, tt, f >> 1, f & 1);
+          for (int f = 0; f < I; ++f)
+            sm.acc[wv][(ht * T + tt) * I + f][lane] = item4(ht, tt, f);
         if (g == 0) sm.ml[wv][ht * 16 + i16] = (f2_t){M[ht], L[ht]};
       }
     };
@@ -780,14 +907,15 @@ __device__ __forceinline__ void decode_int4_body(
 #pragma unroll
       for (int tt = 0; tt < T; ++tt)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < I; ++i) {
+          const int n0 = MODE != kWhole ? 0 : 4 * (i & 1), r = MODE != kWhole ? i : i >> 1;
           f4_t s;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = acc[ht][tt][4 * (i & 1) + e][i >> 1] * own;
+          for (int e = 0; e < 4; ++e) s[e] = acc[ht][tt][n0 + e][r] * own;
 #pragma unroll
-          for (int k = 0; k < K; ++k) s += sm.acc[slot[k]][(ht * T + tt) * 8 + i][lane] * f[k];
+          for (int k = 0; k < K; ++k) s += sm.acc[slot[k]][(ht * T + tt) * I + i][lane] * f[k];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[ht][tt][4 * (i & 1) + e][i >> 1] = s[e];
+          for (int e = 0; e < 4; ++e) acc[ht][tt][n0 + e][r] = s[e];
         }
     }
   };
@@ -821,8 +949,8 @@ __device__ __forceinline__ void decode_int4_body(
 #pragma unroll
       for (int tt = 0; tt < T; ++tt)
 #pragma unroll
-        for (int f = 0; f < 8; ++f)
-          dev_store4(rs, (((ht * T + tt) * 8 + f) * kWave + lane) * 16, piece4(ht, tt, f >> 1, f & 1));
+        for (int f = 0; f < I; ++f)
+          dev_store4(rs, (((ht * T + tt) * I + f) * kWave + lane) * 16, item4(ht, tt, f));
       if (g == 0) {
         const f2_t ml = {M[ht], L[ht]};
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2_t, ml), rs,
@@ -833,12 +961,12 @@ __device__ __forceinline__ void decode_int4_body(
   };
   // Four dims of a head (item f of a piece) as outputs.
   auto store_item = [&](int seq, int kvh, int ch, int f, f4_t s, float l) {
-    const int hh = ch * 16 * HT + (f / (8 * T)) * 16 + i16;
-    const int chunk = ((f / 8) % T) * 16 + 4 * g + ((f & 7) >> 1);
+    const int hh = ch * 16 * HT + item_head(f) * 16 + column;
+    const int chunk = item_chunk(f);
     if (hh >= sh.group || chunk >= C) return;
     const float inv = l != 0.f ? 1.f / l : 0.f;
     *reinterpret_cast<uint2*>(out + ((size_t)seq * sh.num_heads + kvh * sh.group + hh) * D +
-                              chunk * 8 + 4 * (f & 1)) =
+                              chunk * 8 + 4 * item_half(f)) =
         make_uint2(pack2<BF>(s[0] * inv, s[1] * inv), pack2<BF>(s[2] * inv, s[3] * inv));
   };
   auto note_shared = [&](int which, const I4Unit& u) {
@@ -865,7 +993,8 @@ __device__ __forceinline__ void decode_int4_body(
       const int which = begun ? 1 : 0;
 #pragma unroll
       for (int q2 = 0; q2 < T * HT; ++q2) {
-        const int f = wv + q2 * kI4Waves, h = (f / (8 * T)) * 16 + i16;
+        const int f = wv + q2 * kI4Waves, h = item_head(f) * 16 + i16;
+        if (f >= G::NF) break;
         f2_t ml[kI4Waves];
         f4_t v[kI4Waves];
         float mx = kNegInf, l = 0.f;
@@ -889,7 +1018,7 @@ __device__ __forceinline__ void decode_int4_body(
           const auto rs = buf_rsrc(ws + (size_t)(2 * b + which) * G::kSlotFloats,
                                    (uint32_t)(G::kSlotFloats * 4));
           dev_store4(rs, (f * kWave + lane) * 16, s);
-          if (f % (8 * T) == 0 && g == 0) {
+          if (f % (I * T) == 0 && g == 0) {
             const f2_t p = {mx, l};
             __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2_t, p), rs,
                                                   G::kPieceFloats * 4 + h * 8, 0, kPolicyDevice);
@@ -953,8 +1082,9 @@ __device__ __forceinline__ void decode_int4_body(
     float Mi[T * HT], Li[T * HT];
 #pragma unroll
     for (int q = 0; q < T * HT; ++q) {
-      const int f = wv + q * kI4Waves;                  // (ht * T + tt) * 8 + 2 r + half
-      const int h = (f / (8 * T)) * 16 + i16;
+      const int f = wv + q * kI4Waves;
+      const int h = item_head(f) * 16 + i16;
+      if (f >= G::NF) break;
       float mx = kNegInf, l = 0.f;
       f4_t s = {0.f, 0.f, 0.f, 0.f};
       for (int j0 = 0; j0 < n; j0 += K) {
@@ -988,7 +1118,7 @@ __device__ __forceinline__ void decode_int4_body(
     if (final_out) {
 #pragma unroll
       for (int q = 0; q < T * HT; ++q)
-        store_item(seq, kvh, ch, wv + q * kI4Waves, A[q], Li[q]);
+        if (wv + q * kI4Waves < G::NF) store_item(seq, kvh, ch, wv + q * kI4Waves, A[q], Li[q]);
     } else {
       // (each thread rewrites the items that it alone read; the pairs, which all read, after
       // a barrier)
@@ -997,12 +1127,13 @@ __device__ __forceinline__ void decode_int4_body(
 #pragma unroll
       for (int q = 0; q < T * HT; ++q) {
         const int f = wv + q * kI4Waves;
+        if (f >= G::NF) break;
         dev_store4(rs, (f * kWave + lane) * 16, A[q]);
-        if (f % (8 * T) == 0 && g == 0) {
+        if (f % (I * T) == 0 && g == 0) {
           const f2_t ml = {Mi[q], Li[q]};
           __builtin_amdgcn_raw_buffer_store_b64(
               __builtin_bit_cast(u2_t, ml), rs,
-              G::kPieceFloats * 4 + ((f / (8 * T)) * 16 + i16) * 8, 0, kPolicyDevice);
+              G::kPieceFloats * 4 + (item_head(f) * 16 + i16) * 8, 0, kPolicyDevice);
         }
       }
     }
@@ -1049,7 +1180,7 @@ __device__ __forceinline__ void decode_int4_body(
 //
 // The first arguments reach the waves in registers; the lengths are loaded while the rest come, whether
 // the call is checked among the first.
-template <int STEPS, int MAX_HT, bool BF>
+template <int STEPS, int MAX_HT, int MODE, bool BF>
 __global__ void __launch_bounds__(kI4Waves* kWave) __attribute__((amdgpu_waves_per_eu(2)))
 decode_int4_kernel(const int32_t* __restrict__ lengths, int num_seqs, int max_blocks, int bs_check,
                    int num_kv_heads, int group, int head_dim, int num_blocks, float scale_log2,
@@ -1061,7 +1192,7 @@ decode_int4_kernel(const int32_t* __restrict__ lengths, int num_seqs, int max_bl
   const int bs_log2 = bs_check & 255;
   const Int4DecodeShape sh{num_seqs, num_kv_heads * group, num_kv_heads, group, head_dim, num_blocks,
                            max_blocks, bs_log2, scale_log2};
-  __shared__ I4Smem<STEPS, MAX_HT> sm;
+  __shared__ I4Smem<STEPS, MAX_HT, MODE> sm;
   const const_i32 ctxl = as_const(lengths), bt = as_const(table);
   const I4Lens lens = i4_lens(ctxl, sh.num_seqs, sh.max_blocks << sh.bs_log2);
   // A checked call's answer goes out at once, while the launch goes on; all leave where it is no.
@@ -1073,19 +1204,19 @@ decode_int4_kernel(const int32_t* __restrict__ lengths, int num_seqs, int max_bl
   }
   if constexpr (MAX_HT > 1) {
     if (lens.total * (uint32_t)sh.num_kv_heads >= kI4TwoTiles) {
-      decode_int4_body<STEPS, 2, BF>(sm, lens, bt, ctxl, sh, q, kc, vc, ks, vs, out, ws, cnt);
+      decode_int4_body<STEPS, 2, kWhole, BF>(sm, lens, bt, ctxl, sh, q, kc, vc, ks, vs, out, ws, cnt);
       return;
     }
   }
-  decode_int4_body<STEPS, 1, BF>(reinterpret_cast<I4Smem<STEPS, 1>&>(sm), lens, bt, ctxl, sh, q, kc,
+  decode_int4_body<STEPS, 1, MODE, BF>(reinterpret_cast<I4Smem<STEPS, 1, MODE>&>(sm), lens, bt, ctxl, sh, q, kc,
                                  vc, ks, vs, out, ws, cnt);
 }
 
 namespace {
 
-template <int MAX_HT, bool BF>
+template <int MAX_HT, int MODE, bool BF>
 hipError_t launch_tiles(const Int4Decode& l) {
-  decode_int4_kernel<PA_INT4_STEPS, MAX_HT, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
+  decode_int4_kernel<PA_INT4_STEPS, MAX_HT, MODE, BF><<<kI4Groups, kI4Waves * kWave, 0, l.stream>>>(
       l.context_lens, l.shape.num_seqs, l.shape.max_blocks,
       l.shape.bs_log2 | (l.report != nullptr ? kI4Check : 0), l.shape.num_kv_heads, l.shape.group,
       l.shape.head_dim, l.shape.num_blocks, l.shape.scale_log2, l.block_table,
@@ -1101,15 +1232,23 @@ hipError_t launch_tiles(const Int4Decode& l) {
 template <>
 hipError_t launch_int4_decode_steps<PA_INT4_STEPS>(const Int4Decode& l) {
 #if PA_INT4_STEPS <= 4
-  if (l.shape.group > 16) return l.bf16 ? launch_tiles<2, true>(l) : launch_tiles<2, false>(l);
+  if (l.shape.group > 16)
+    return l.bf16 ? launch_tiles<2, kWhole, true>(l) : launch_tiles<2, kWhole, false>(l);
 #endif
-  return l.bf16 ? launch_tiles<1, true>(l) : launch_tiles<1, false>(l);
+#if PA_INT4_STEPS > 2
+  if (l.shape.group <= 4)
+    return l.bf16 ? launch_tiles<1, kPack4, true>(l) : launch_tiles<1, kPack4, false>(l);
+#endif
+  constexpr int kFewHeads = PA_INT4_STEPS <= 2 ? kPair : kPack;
+  if (l.shape.group <= 8)
+    return l.bf16 ? launch_tiles<1, kFewHeads, true>(l) : launch_tiles<1, kFewHeads, false>(l);
+  return l.bf16 ? launch_tiles<1, kWhole, true>(l) : launch_tiles<1, kWhole, false>(l);
 }
 
 template <>
 size_t int4_decode_slot_bytes<PA_INT4_STEPS>(int group) {
-  return sizeof(float) * (PA_INT4_STEPS <= 4 && group > 16 ? I4Geo<PA_INT4_STEPS, 2>::kSlotFloats
-                                                           : I4Geo<PA_INT4_STEPS, 1>::kSlotFloats);
+  return sizeof(float) * (PA_INT4_STEPS <= 4 && group > 16 ? I4Geo<PA_INT4_STEPS, 2, kWhole>::kSlotFloats
+                                                           : I4Geo<PA_INT4_STEPS, 1, kWhole>::kSlotFloats);
 }
 
 }  // namespace pa

@@ -317,6 +317,15 @@ def test_decode_group_sizes(heads, hkv, d):
     check_decode([130, 1, 67], heads, hkv, d, 16, torch.float16, heads + d)
 
 
+@pytest.mark.parametrize("heads,hkv", [(2, 1), (8, 2), (10, 2), (8, 1), (18, 2)])
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 128, 136, 200, 256])
+@pytest.mark.parametrize("lens", [[20000, 3, 0, 700], [513, 64, 8, 9, 17]])
+def test_decode_small_groups_of_every_width(heads, hkv, d, lens):
+    """Groups of 2, 4, 5, 8 and 9 heads, whose unused columns hold parts of the work; pieces
+    of one work-group and of many."""
+    check_decode(lens, heads, hkv, d, 16, torch.bfloat16 if d % 16 else torch.float16, heads + d)
+
+
 @pytest.mark.parametrize("lens", [
     [4096] * 4, [20000], [20000, 1, 3, 9000], list(range(1, 130)), [1] * 300,
     [0, 5, 0, 0, 700, 0], [0], [0, 0, 0],
