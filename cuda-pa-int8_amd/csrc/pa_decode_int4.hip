@@ -46,8 +46,8 @@
 // (lengths, block ids, rows: three loads that wait for each other) and 5 to 9 us from the last
 // rows to the end where units are shared between work-groups, which is what bounds short ones.
 // Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 6.7; 32 x 4096, 12/2 of 128: 14.0 (36 MB);
-// 8 x 32768, 32/8 of 128: 55 (5.2 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
-// 32/8 of 128: 65 (5.1 TB/s); 24 x 900-9000, 8/4 of 256: 33.2 (4.7 TB/s).
+// 8 x 32768, 32/8 of 128: 54 (5.3 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
+// 32/8 of 128: 64 (5.2 TB/s); 24 x 900-9000, 8/4 of 256: 33.2 (4.7 TB/s).
 #include <math.h>
 
 #include "pa_decode_kernels.hpp"
