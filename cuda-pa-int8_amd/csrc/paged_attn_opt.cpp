@@ -493,6 +493,8 @@ void reshape_and_cache_int4(at::Tensor key, at::Tensor value, at::Tensor k_cache
                             at::Tensor v_cache, at::Tensor k_scales, at::Tensor v_scales,
                             at::Tensor slot_mapping) {
   check_int4_rows(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping);
+  TORCH_CHECK(k_cache.data_ptr() != v_cache.data_ptr() && k_scales.data_ptr() != v_scales.data_ptr(),
+              "the caches of key and value must not be one tensor");
   const at::hip::HIPGuardMasqueradingAsCUDA guard(key.device());
   hipStream_t stream = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(key.get_device()).stream();
   check_status(pa_reshape_and_cache_int4(
@@ -521,6 +523,8 @@ void gather_cache_int4(at::Tensor key, at::Tensor value, at::Tensor k_cache, at:
   check_int4_rows(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping);
   for (const at::Tensor* t : {&key, &value})
     TORCH_CHECK(rows_disjoint(*t), "the rows of key and value must not overlap");
+  TORCH_CHECK(key.numel() == 0 || key.data_ptr() != value.data_ptr(),
+              "key and value must not be one tensor");
   const at::hip::HIPGuardMasqueradingAsCUDA guard(key.device());
   hipStream_t stream = at::hip::getCurrentHIPStreamMasqueradingAsCUDA(key.get_device()).stream();
   check_status(pa_gather_cache_int4(

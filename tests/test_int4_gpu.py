@@ -243,6 +243,22 @@ def test_write_of_nothing_and_all_skipped():
     assert all(torch.equal(a, b) for a, b in zip(got, keep))
 
 
+def test_one_tensor_for_key_and_value_is_refused():
+    import pa_int8
+
+    kc, vc, ks, vs = new_cache(2, 2, 64, 16, fill=0.5)
+    k, i = torch.ones(5, 2, 64, dtype=torch.float16, device=DEV), torch.arange(5, device=DEV)
+    pa_int8.reshape_and_cache_int4(k, k, kc, vc, ks, vs, i)      # (as rows to write it is fine)
+    for caches in ((kc, kc, ks, vs), (kc, vc, ks, ks)):
+        with pytest.raises(RuntimeError, match="one tensor"):
+            pa_int8.reshape_and_cache_int4(k, k, *caches, i)
+    with pytest.raises(RuntimeError, match="one tensor"):
+        pa_int8.gather_cache_int4(k, k, kc, vc, ks, vs, i)
+    out = torch.empty(2, 5, 2, 64, dtype=torch.float16, device=DEV)
+    pa_int8.gather_cache_int4(out[0], out[1], kc, kc, ks, ks, i)  # (one cache read twice, too)
+    assert bool((out == 1).all())
+
+
 # ------------------------------------------------------------------ decode
 
 def paged(lens, hkv, d, bs, dtype, seed, k_mul=1.0, v_mul=1.0, spread=0.0, extra_cols=0):
