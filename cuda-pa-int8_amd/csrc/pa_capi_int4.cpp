@@ -56,10 +56,10 @@ pa_status_t decode_shape(int32_t num_seqs, int32_t num_heads, int32_t head_dim,
   if (num_seqs < 0 || num_heads < 1 || num_heads % num_kv_heads != 0 || max_blocks < 0 ||
       (int64_t)max_blocks * block_size > INT32_MAX - 128)
     return PA_ERR_BAD_SHAPE;
-  // The kernel counts two parts a 64-token tile and one more for every (sequence, kv head, chunk
-  // of query heads) in 31 bits.
-  const int64_t parts = 2 * ((int64_t)max_blocks * block_size / 64 + 1) + 1;
-  if (num_seqs > INT32_MAX / num_heads || (int64_t)num_seqs * num_heads > INT32_MAX / parts)
+  // The kernel counts the 64-token tiles of every (sequence, kv head, chunk of query heads) in 31
+  // bits.
+  const int64_t tiles = (int64_t)max_blocks * block_size / 64 + 1;
+  if (num_seqs > INT32_MAX / num_heads || (int64_t)num_seqs * num_heads > INT32_MAX / tiles)
     return PA_ERR_BAD_SHAPE;
   *s = pa::Int4DecodeShape{num_seqs, num_heads, num_kv_heads, num_heads / num_kv_heads, head_dim,
                            num_blocks, max_blocks, __builtin_ctz((unsigned)block_size),

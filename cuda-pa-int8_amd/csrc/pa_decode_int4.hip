@@ -32,9 +32,8 @@
 // Work.  The tiles of all units (sequence, kv head, chunk of 16 HT query heads) form one list,
 // in that order.  It is divided evenly among the work-groups, one a CU, and a work-group's part
 // among its waves: as even as tiles are, whatever the lengths, and found by every wave from
-// context_lens alone.  (Where lengths differ and the list is long, by cost rather than by tiles;
-// where units are few and short, a work-group takes one unit: both below.)  A unit inside one
-// wave's range needs no merge at all; the pieces of a unit that several waves share are merged
+// context_lens alone.  (Where units are few and short, a work-group takes one unit.)  A unit
+// inside one wave's range needs no merge at all; the pieces of a unit that several waves share are merged
 // through LDS, and those of a unit that several work-groups share through memory, by the last of
 // them to arrive (in two levels above kMergeMax pieces).  All orders are fixed: the same bits
 // every time.
@@ -45,9 +44,9 @@
 // is behind goes first on its SIMD.  A launch has about 2.5 us before its first rows arrive
 // (lengths, block ids, rows: three loads that wait for each other) and 5 to 9 us from the last
 // rows to the end where units are shared between work-groups, which is what bounds short ones.
-// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 6.7; 32 x 4096, 12/2 of 128: 14.0 (36 MB);
+// Measured, in us: 4 x 100-512 tokens, 8/8 heads of 64: 6.6; 32 x 4096, 12/2 of 128: 13.6 (36 MB);
 // 8 x 32768, 32/8 of 128: 54 (5.3 TB/s); 192 ragged sequences (median 1024 tokens, at most 8192),
-// 32/8 of 128: 64 (5.2 TB/s); 24 x 900-9000, 8/4 of 256: 33.2 (4.7 TB/s).
+// 32/8 of 128: 65 (5.1 TB/s); 24 x 900-9000, 8/4 of 256: 32.8 (4.7 TB/s).
 #include <math.h>
 
 #include "pa_decode_kernels.hpp"
@@ -239,13 +238,12 @@ struct I4Lens {
   int per, lane_ctx;        // sequences a lane; the context of the lane's last
   uint32_t incl, total;     // tiles of one (kv head, chunk): the lanes' running sum, and all
   uint32_t longest;         // tiles of a sequence: the longest of this lane's
-  bool ragged;              // whether sequences differ
   bool empty;               // whether one holds no token
 };
 __device__ __forceinline__ I4Lens i4_lens(const_i32 ctxl, int S, int cap) {
   I4Lens r;
   r.per = (S + kWave - 1) / kWave;
-  uint32_t mine = 0, shortest = ~0u;
+  uint32_t mine = 0;
   r.longest = 0;
   r.lane_ctx = 0;
   int least = 1;
@@ -256,13 +254,10 @@ __device__ __forceinline__ I4Lens i4_lens(const_i32 ctxl, int S, int cap) {
     r.lane_ctx = i4_clamp_ctx(ctx, cap);
     const uint32_t n = i4_tiles(r.lane_ctx);
     mine += s < S ? n : 0u;
-    shortest = min(shortest, n);
     r.longest = max(r.longest, n);
   }
   r.incl = wave_scan_dpp(mine);
   r.total = (uint32_t)__builtin_amdgcn_readlane((int)r.incl, kWave - 1);
-  const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)shortest);
-  r.ragged = __any(shortest != first || r.longest != first);
   r.empty = __any(least < 1);
   return r;
 }
@@ -295,13 +290,6 @@ __device__ __forceinline__ void decode_int4_body(
   const int per = lens.per, lane_ctx = lens.lane_ctx;
   const uint32_t incl = lens.incl;
   const uint32_t tiles = lens.total * (uint32_t)U;
-  // The list is divided by cost: 2 for a tile and 1 for a unit's start and end, where the units
-  // differ and a wave has tiles enough to make up for it (192 sequences of median 1024 and at most
-  // 8192 tokens 71.7 -> 65 us, 512 of 20 to 200 29.4 -> 28.6); else evenly by tiles, as equal units
-  // divide best (32 x 4096 by cost 16.3 -> 19.0).
-  const bool weigh = lens.ragged && tiles >= 4u * kI4Groups * kI4Waves;
-  const uint32_t tile_cost = weigh ? 2u : 1u, unit_cost = weigh ? 1u : 0u;
-  const uint32_t W = tiles * tile_cost + (uint32_t)(S * U) * unit_cost;
   // (another work-group as soon as every wave has a tile: with two each, 2000 tokens at 28/4 heads
   // 10.7 -> 13.0 us)
   const uint32_t want = (tiles + kI4Waves - 1) / kI4Waves;
@@ -313,21 +301,20 @@ __device__ __forceinline__ void decode_int4_body(
   const uint32_t groups = whole ? units : (want < kI4Groups ? want : kI4Groups);
   const uint32_t b = blockIdx.x;
   if (b >= groups) return;
-  // Work-group b takes W / groups of the cost, the first W % groups one more; its waves
-  // likewise.  A point of the list at cost x stands for the tile there (a unit's first, at
-  // its start).
-  const uint32_t Q = W / groups, R = W - Q * groups;
+  // Work-group b takes tiles / groups tiles of the list, the first tiles % groups one more; its
+  // waves likewise.  (Divided by cost, half a tile for a unit's start and end, 192 ragged sequences
+  // ran 66.1 -> 65.0 us and the other calls 0.2 us longer.)
+  const uint32_t Q = tiles / groups, R = tiles - Q * groups;
   const uint32_t gn = Q + (b < R ? 1u : 0u);
   const uint32_t x0 = b * Q + min(b, R) + wv * (gn / kI4Waves) + min((uint32_t)wv, gn % kI4Waves);
   const uint32_t x1 = x0 + gn / kI4Waves + ((uint32_t)wv < gn % kI4Waves ? 1u : 0u);
 
-  // The tile at cost x < W (where its unit starts, in `begin`), and its index in the list.
-  const uint32_t lane_seqs = (uint32_t)min((lane + 1) * per, S);
-  const uint32_t lane_cost = (incl * tile_cost + lane_seqs * unit_cost) * (uint32_t)U;
-  auto tile_at = [&](uint32_t x, I4Tile& t, uint32_t& begin) {
+  // Tile x of the list, and where its unit starts.
+  const uint32_t lane_end = incl * (uint32_t)U;
+  auto tile_at = [&](uint32_t x, I4Tile& t) {
     // The sequence: its lane by a ballot, then, where a lane has several, a walk over that
     // lane's.
-    const unsigned long long before = __ballot(lane_cost <= x);
+    const unsigned long long before = __ballot(lane_end <= x);
     const int l = min((int)__builtin_popcountll(before), kWave - 1);
     uint32_t base = l > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)incl, l - 1) : 0u;
     int s = min(l * per, S - 1), n, ctx;
@@ -339,29 +326,24 @@ __device__ __forceinline__ void decode_int4_body(
       for (int j = 0;; ++j) {
         ctx = i4_clamp_ctx(ctxl[s], cap);
         n = i4_tiles(ctx);
-        if (j >= per - 1 || s >= S - 1 ||
-            ((base + n) * tile_cost + (uint32_t)(s + 1) * unit_cost) * U > x)
-          break;
+        if (j >= per - 1 || s >= S - 1 || (base + n) * U > x) break;
         base += n;
         ++s;
       }
       t.ctx_next = ctxl[min(s + 1, S - 1)];
     }
-    const uint32_t unit = (uint32_t)n * tile_cost + unit_cost;
-    const uint32_t in = x - (base * tile_cost + (uint32_t)s * unit_cost) * U, u = in / unit;
-    const uint32_t c = in - u * unit;
-    begin = x - c;
+    const uint32_t in = x - base * U, u = in / (uint32_t)n;
     t.seq = s;
     t.ctx = ctx;
     t.n = n;
-    t.t = c < unit_cost ? 0 : (int)((c - unit_cost) / tile_cost);
+    t.t = (int)(in - u * n);
     t.kvh = (int)(u / (uint32_t)nchunk);
     t.ch = (int)u - t.kvh * nchunk;
-    return base * U + u * n + (uint32_t)t.t;
+    return x - (uint32_t)t.t;
   };
-  I4Tile cur, after;
-  uint32_t unit0 = 0, unit1 = W;     // where the units at both ends of the range start
-  int count;
+  I4Tile cur;
+  uint32_t unit0 = 0;                // where the first tile's unit starts
+  int count = (int)(x1 - x0);
   if (whole) {
     const int seq = (int)(b / (uint32_t)U), u = (int)b - seq * U;
     cur.seq = seq;
@@ -373,8 +355,7 @@ __device__ __forceinline__ void decode_int4_body(
     cur.t = wv * (cur.n / kI4Waves) + min(wv, cur.n % kI4Waves);
     count = cur.n / kI4Waves + (wv < cur.n % kI4Waves ? 1 : 0);
   } else {
-    const uint32_t tile0 = tile_at(x0, cur, unit0);
-    count = (int)((x1 < W ? tile_at(x1, after, unit1) : tiles) - tile0);
+    unit0 = tile_at(x0, cur);
   }
 
   auto advance = [&](I4Tile& t) {
@@ -859,7 +840,7 @@ __device__ __forceinline__ void decode_int4_body(
     finish(cur.t == cur.n - 1, (state & kHead) && cur.t == t0 + count - 1);
     if (kTogether && (state & (kHead | kTail)) == kTail) {
       to_slot();
-      if (lane == 0) sm.tail[wv] = I4Unit{unit1, cur.n, cur.seq, cur.kvh, cur.ch};
+      if (lane == 0) sm.tail[wv] = I4Unit{x1 - 1 - cur.t, cur.n, cur.seq, cur.kvh, cur.ch};
     }
   }
   if (lane == 0) sm.state[wv] = state;
@@ -972,9 +953,8 @@ __device__ __forceinline__ void decode_int4_body(
   auto note_shared = [&](int which, const I4Unit& u) {
     auto& p = sm.piece[which];
     p.active = 1;
-    // (the points that stand for the unit's first tile, and all of the unit's)
-    p.first = worker_group(u.begin + unit_cost + tile_cost - 1);
-    p.count = worker_group(u.begin + unit_cost + u.n * tile_cost - 1) - p.first + 1;
+    p.first = worker_group(u.begin);
+    p.count = worker_group(u.begin + u.n - 1) - p.first + 1;
     p.seq = u.seq;
     p.kvh = u.kvh;
     p.ch = u.ch;
@@ -1036,7 +1016,7 @@ __device__ __forceinline__ void decode_int4_body(
         write_out(cur.seq, cur.kvh, cur.ch);
       } else {
         share(1);
-        if (lane == 0) note_shared(1, I4Unit{unit1, cur.n, cur.seq, cur.kvh, cur.ch});
+        if (lane == 0) note_shared(1, I4Unit{x1 - 1 - cur.t, cur.n, cur.seq, cur.kvh, cur.ch});
       }
     }
     if (wv == 0 && lead != 0) {
